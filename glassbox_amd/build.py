@@ -59,6 +59,9 @@ LIBRARIES: Dict[str, tuple] = {
     "groupmix": ("hip", ["hip/groupmix.hip"], ["hip/common.h"]),
     "delta": ("hip", ["hip/delta.hip"], ["hip/common.h"]),
     "latent": ("hip", ["hip/latent.hip"], ["hip/common.h"]),
+    "fp4_cache": ("hip", ["hip/fp4_cache.hip"], ["hip/common.h", "hip/fp4.h"]),
+    "fp4_attention": ("hip", ["hip/fp4_attention.hip"], ["hip/common.h", "hip/fp4.h"]),
+    "fp4_gemm": ("hip", ["hip/fp4_gemm.hip"], ["hip/common.h", "hip/fp4.h"]),
 }
 
 _lock = threading.Lock()

@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import struct
-from typing import List, Optional, Sequence
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -270,6 +270,28 @@ _SIGS = {
                                            _i, _i, _vp],
         "gb_attention_prefill_bf16_out32": [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i,
                                             _f, _i, _i, _i, _i, _vp, C.c_longlong, _vp],
+    },
+    "fp4_cache": {
+        # qkv, dtype, stride, q, its stride, cos, sin, slots, k, v, n, nh, nkv, hd, page, pages, stream
+        "gb_fp4_store": [_vp, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
+        # slots, k pages, v pages, k, its stride, v, its stride, dtype, n, nkv, hd, page, pages, stream
+        "gb_fp4_load": [_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp],
+        # w, dtype, stride, codes, scales, n, k, scales a row, stream
+        "gb_fp4_quantize": [_vp, _i, _i, _vp, _vp, _i, _i, _i, _vp],
+        # codes, scales, w, dtype, n, k, scales a row, stream
+        "gb_fp4_expand": [_vp, _vp, _vp, _i, _i, _i, _i, _vp],
+    },
+    "fp4_attention": {
+        # q, stride, out, stride, dtype, n, q_start, q_len, pos0, requests, longest, max_context, tables, stride, columns, k, v, pages,
+        # nh, nkv, hd, page, scale, window, workspace, its floats, stream
+        "gb_fp4_attention": [_vp, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _i,
+                             _vp, C.c_longlong, _vp],
+        "gb_fp4_attention_floats": [_i, _i, _i, _i, _i, _i, _i, _i],
+        "gb_fp4_attention_takes": [_i],
+    },
+    "fp4_gemm": {
+        # a, dtype, lda, codes, scales, scales a row, out, its dtype, ldo, M, N, K, epilogue, stream
+        "gb_fp4_gemm": [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp],
     },
     "sampling": {
         "gb_argmax": [_vp, _vp, _i, _i, _vp],
@@ -2544,3 +2566,227 @@ def delta_chunk_floats(rows: int, n_seqs: int, n_heads: int, key_dim: int, value
     f = _lib("delta").gb_delta_chunk_floats
     f.restype = C.c_longlong
     return int(f(rows, n_seqs, n_heads, key_dim, value_dim))
+
+
+# ------------------------------------------------------------------------ numbers of four bits
+# Blocks of 32 neighbouring numbers share a power of two, 2^(b - 127) with b a byte; a number is sign and one of 0, 0.5, 1, 1.5, 2, 3,
+# 4, 6 times that (csrc/hip/fp4.h): 4.25 bits a number.  They hold keys and values of a cache (blocks of a head's channels) and
+# matrices (blocks of the inner size).  A block with a number that is infinite or NaN reads as NaN.
+FP4_BLOCK = 32
+FP4_HEAD_DIMS = (32, 64, 96, 128, 256)   # heads that ``fp4_attention`` takes
+
+
+class Fp4Matrix(NamedTuple):
+    """A matrix of four-bit numbers.  ``codes``: uint8 [rows, columns / 2], byte i of a row numbers 2i (low half) and 2i + 1, bit 3 of a
+    number its sign; ``scales``: uint8 [rows, columns / 32 filled up to a multiple of 16], a byte a block.  Both contiguous."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.codes.shape[0], 2 * self.codes.shape[1]
+
+
+def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The operands lie on the current device, whose stream the kernels are launched on."""
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.get_device() != _get_device()):
+            raise KernelError(f"{what}: operands must be on the current GPU")
+
+
+def _span(t: torch.Tensor):
+    at = t.data_ptr()
+    return at, at + (1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else at
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor, what: str, same: bool = False) -> None:
+    """The two share no memory; with ``same`` they may be rows at the same places."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a0 < b1 and b0 < a1 and not (same and a0 == b0 and a.stride() == b.stride()):
+        raise KernelError(what)
+
+
+def fp4_scale_bytes(columns: int) -> int:
+    """Scales that a row of a matrix of so many columns has (``Fp4Matrix.scales``)."""
+    return -(-(columns // FP4_BLOCK) // 16) * 16
+
+
+def fp4_pages_shape(pages: int, n_kv_heads: int, page_size: int, head_dim: int) -> tuple:
+    """Shape of four-bit key pages and of value pages (uint8): [pages, kv heads, head size / 32, 17, page size].  Of a block of 32 channels the
+    first 16 x page size bytes are the codes (keys: 16 bytes a slot; values: byte rows of channels i and i + 16 over the slots),
+    the last row the slots' scales.  All bytes zero: values of zero."""
+    return (pages, n_kv_heads, head_dim // FP4_BLOCK, 17, page_size)
+
+
+def _fp4_pages(k_pages, v_pages, what: str):
+    """(pages, kv heads, page size, head size) of four-bit pages."""
+    if (k_pages is None or v_pages is None or k_pages.dim() != 5 or k_pages.shape != v_pages.shape or k_pages.shape[3] != 17
+            or k_pages.shape[4] % 16 or 0 in k_pages.shape or k_pages.dtype != torch.uint8 or v_pages.dtype != torch.uint8
+            or not k_pages.is_contiguous() or not v_pages.is_contiguous() or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16):
+        raise KernelError(f"{what}: four-bit pages are contiguous uint8 [pages, kv heads, head size / 32, 17, page size], of a multiple of "
+                          f"16 slots, keys and values alike")
+    p, h, nb, _, s = k_pages.shape
+    return p, h, s, nb * FP4_BLOCK
+
+
+def fp4_store(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], slots: Optional[torch.Tensor],
+              k_pages: Optional[torch.Tensor], v_pages: Optional[torch.Tensor], n_heads: int, n_kv_heads: int, head_dim: int,
+              q: Optional[torch.Tensor] = None) -> None:
+    """What ``rope_store`` does, into four-bit pages: each stacked row's query heads are turned by its angles (``cos``, ``sin`` float32
+    [n, head size / 2]; None: nothing is turned) and written to ``q`` [n, heads * head size] (None: back where they were); its key heads,
+    turned in 32 bits, and its value heads go to the pages at ``slots`` as the nearest four-bit numbers.  The keys and values of ``qkv``
+    are left as they are.  ``slots`` None: nothing is stored.  A row whose slot is negative or beyond the pages is not stored; the slots of
+    the others must differ."""
+    n = qkv.shape[0]
+    stride = _rows(qkv, "qkv")
+    width = (n_heads + 2 * n_kv_heads) * head_dim
+    if n_heads < 0 or n_kv_heads < 0 or head_dim <= 0 or head_dim % FP4_BLOCK:
+        raise KernelError(f"fp4_store: {n_heads} and {n_kv_heads} heads of {head_dim} channels: a multiple of {FP4_BLOCK} is needed")
+    if qkv.shape[1] < width:
+        raise KernelError(f"fp4_store: rows of {qkv.shape[1]} do not hold {n_heads} + 2 * {n_kv_heads} heads of {head_dim}")
+    pages = page_size = 0
+    if slots is not None:
+        _i32(slots, "slots", n)
+        pages, p_heads, page_size, p_hd = _fp4_pages(k_pages, v_pages, "fp4_store")
+        if (p_heads, p_hd) != (n_kv_heads, head_dim):
+            raise KernelError("fp4_store: pages do not have this layer's kv heads and head size")
+    if (cos is None) != (sin is None):
+        raise KernelError("fp4_store: cosines and sines go together")
+    for t in (cos, sin):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or t.shape[0] < n or t.shape[1] != head_dim // 2):
+            raise KernelError("fp4_store: cos/sin must be contiguous float32 [n, head_dim/2]")
+    if q is None:
+        q, q_stride = qkv, stride
+    else:
+        q_stride = _rows(q, "q")
+        if q.dtype != qkv.dtype or q.shape != (n, n_heads * head_dim):
+            raise KernelError(f"fp4_store: q must be [{n}, {n_heads * head_dim}] of the rows' type")
+        _apart(q, qkv, "fp4_store: q lies over other columns of the rows", same=True)
+    dtype = dtype_code(qkv)
+    _here("fp4_store", qkv, cos, sin, slots, k_pages, v_pages, q)
+    lib = _lib("fp4_cache")
+    _launch(lib, lib.gb_fp4_store, _p(qkv), dtype, stride, _p(q), q_stride, _p(cos), _p(sin), _p(slots), _p(k_pages), _p(v_pages),
+            n, n_heads, n_kv_heads, head_dim, page_size, pages, _stream())
+
+
+def fp4_load(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    """The keys and values that four-bit pages hold at ``slots``, as the values they stand for: ``k``, ``v`` [n, kv heads * head size],
+    bfloat16 (exact) or float32.  Rows whose slot is negative or beyond the pages are left as they are."""
+    pages, nkv, page_size, hd = _fp4_pages(k_pages, v_pages, "fp4_load")
+    n = k.shape[0]
+    _i32(slots, "slots", n)
+    if k.dtype != v.dtype or k.shape != (n, nkv * hd) or v.shape != (n, nkv * hd):
+        raise KernelError(f"fp4_load: k and v must be [{n}, {nkv * hd}] of one type")
+    _apart(k, v, "fp4_load: k and v share memory")
+    dtype, k_stride, v_stride = dtype_code(k), _rows(k, "k"), _rows(v, "v")
+    _here("fp4_load", slots, k_pages, v_pages, k, v)
+    lib = _lib("fp4_cache")
+    _launch(lib, lib.gb_fp4_load, _p(slots), _p(k_pages), _p(v_pages), _p(k), k_stride, _p(v), v_stride, dtype, n, nkv, hd, page_size,
+            pages, _stream())
+
+
+@functools.lru_cache(maxsize=4096)   # a pure function of the sizes, asked for at every step
+def fp4_attention_floats(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, max_q_len: int, max_context: int, window: int = 0,
+                         dtype: torch.dtype = torch.bfloat16) -> int:
+    """Floats of workspace that ``fp4_attention`` needs for so many requests of up to ``max_q_len`` rows: 0 where no context is divided."""
+    f = _lib("fp4_attention").gb_fp4_attention_floats
+    f.restype = C.c_longlong
+    return int(f(int(n_seqs), int(n_heads), int(n_kv_heads), int(head_dim), int(max_q_len), int(max_context), int(window),
+                 F32 if dtype == torch.float32 else BF16))
+
+
+def fp4_attention(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor, pos0: torch.Tensor, tables: torch.Tensor,
+                  k_pages: torch.Tensor, v_pages: torch.Tensor, n_heads: int, scale: float, max_q_len: int, max_context: int,
+                  window: int = 0, workspace: Optional[torch.Tensor] = None) -> None:
+    """Attention over four-bit pages, of single tokens and of portions alike.  Request i brings rows ``q_start[i]`` .. of ``q`` [n, heads * head
+    size], ``q_len[i]`` of them, at positions ``pos0[i]`` and on; each reads the request's keys up to its own position (with ``window`` the
+    last so many) through ``tables`` int32 [requests, pages], and ``out`` receives its rows.  Rows of no request are left as they are.
+    ``max_q_len`` and ``max_context`` are at least the most rows and keys a request has; they size the launch.  A row that sees no key (its
+    position is negative, its pages' numbers are none of the pool's) gives zeros; what lies in a masked place, not finite or not, does not
+    matter.  bfloat16 or float32 rows; heads of 32, 64, 96, 128 or 256 channels; a positive scale.
+    ``workspace`` (float32, ``fp4_attention_floats`` elements): needed where that is not 0."""
+    pages, nkv, page_size, hd = _fp4_pages(k_pages, v_pages, "fp4_attention")
+    n = q.shape[0]
+    if q.dtype != out.dtype or q.dim() != 2 or q.shape[1] != n_heads * hd or out.shape != q.shape:
+        raise KernelError(f"fp4_attention: q and out must be [n, {n_heads} heads * {hd}] of one type")
+    if hd not in FP4_HEAD_DIMS or n_heads <= 0 or n_heads % nkv:
+        raise KernelError(f"fp4_attention: {n_heads} query heads of {hd} channels over {nkv} kv heads: heads of {FP4_HEAD_DIMS}, a multiple of the kv heads")
+    if not 0 < scale < float("inf"):
+        raise KernelError(f"fp4_attention: a positive scale is needed, got {scale}")
+    seqs = q_len.numel()
+    for name, t in (("q_start", q_start), ("q_len", q_len), ("pos0", pos0)):
+        _i32(t, name, seqs)
+    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.stride(1) != 1 or tables.shape[0] < seqs or tables.shape[1] == 0:
+        raise KernelError("fp4_attention: block tables must be int32 [requests, pages]")
+    if window < 0 or max_q_len < 0 or max_context < 0:
+        raise KernelError("fp4_attention: a window, a number of rows or a context below 0")
+    _apart(q, out, "fp4_attention: out lies over other rows of q", same=True)
+    if workspace is not None and (workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.data_ptr() % 16):
+        raise KernelError("fp4_attention: the workspace must be contiguous float32 that begins at a 16-byte word")
+    dtype, q_stride, out_stride = dtype_code(q), _rows(q, "q"), _rows(out, "out")
+    _here("fp4_attention", q, out, q_start, q_len, pos0, tables, k_pages, v_pages, workspace)
+    lib = _lib("fp4_attention")
+    _launch(lib, lib.gb_fp4_attention, _p(q), q_stride, _p(out), out_stride, dtype, n, _p(q_start), _p(q_len), _p(pos0), seqs,
+            int(max_q_len), int(max_context), _p(tables), tables.stride(0), tables.shape[1], _p(k_pages), _p(v_pages), pages, n_heads, nkv, hd,
+            page_size, float(scale), int(window), _p(workspace), workspace.numel() if workspace is not None else 0, _stream())
+
+
+def fp4_quantize(w: torch.Tensor) -> Fp4Matrix:
+    """The nearest four-bit matrix to ``w`` [rows, columns], float32 or bfloat16, columns a multiple of 32."""
+    stride = _rows(w, "w")
+    n, k = w.shape
+    if k % FP4_BLOCK or k == 0:
+        raise KernelError(f"fp4_quantize: rows of {k} numbers: a multiple of {FP4_BLOCK} is needed")
+    dtype = dtype_code(w)
+    _here("fp4_quantize", w)
+    m = Fp4Matrix(torch.empty((n, k // 2), dtype=torch.uint8, device=w.device),
+                  torch.empty((n, fp4_scale_bytes(k)), dtype=torch.uint8, device=w.device))
+    lib = _lib("fp4_cache")
+    _launch(lib, lib.gb_fp4_quantize, _p(w), dtype, stride, _p(m.codes), _p(m.scales), n, k, m.scales.shape[1], _stream())
+    return m
+
+
+def _fp4_matrix(w: Fp4Matrix, what: str) -> Tuple[int, int]:
+    codes, scales = w
+    if (codes.dim() != 2 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_contiguous() or not scales.is_contiguous()
+            or codes.shape[1] % 16 or 0 in codes.shape or scales.shape != (codes.shape[0], fp4_scale_bytes(2 * codes.shape[1]))
+            or codes.data_ptr() % 16 or scales.data_ptr() % 16):
+        raise KernelError(f"{what}: a four-bit matrix has contiguous uint8 codes [rows, columns / 2] and scales [rows, columns / 32 filled up to a "
+                          f"multiple of 16], got {tuple(codes.shape)} and {tuple(scales.shape)}")
+    return w.shape
+
+
+def fp4_expand(w: Fp4Matrix, out: torch.Tensor) -> None:
+    """The values of a four-bit matrix: ``out`` [rows, columns], contiguous, bfloat16 (exact) or float32."""
+    n, k = _fp4_matrix(w, "fp4_expand")
+    if out.shape != (n, k) or not out.is_contiguous() or out.data_ptr() % 16:
+        raise KernelError(f"fp4_expand: out must be contiguous [{n}, {k}] and begin at a 16-byte word")
+    dtype = dtype_code(out)
+    _here("fp4_expand", *w, out)
+    lib = _lib("fp4_cache")
+    _launch(lib, lib.gb_fp4_expand, _p(w.codes), _p(w.scales), _p(out), dtype, n, k, w.scales.shape[1], _stream())
+
+
+def fp4_gemm_floats(rows: int, n: int, k: int, dtype: torch.dtype = torch.bfloat16) -> int:
+    """Floats of workspace with which ``fp4_gemm`` is faster for so many rows; 0 if it has no use for any."""
+    return 0
+
+
+def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool = False, silu_mul: bool = False,
+             workspace: Optional[torch.Tensor] = None) -> None:
+    """out (+)= a . w^T with four-bit weights, the sums in 32 bits: ``a`` [rows, columns of w] bfloat16 or float32, ``out`` bfloat16 or float32
+    (float32 when accumulating).  ``silu_mul``: w stacks gate rows over up rows and out[m, j] = silu(a . gate_j) * (a . up_j), of half as
+    many columns.  ``workspace`` (float32, ``fp4_gemm_floats`` elements) is optional."""
+    N, K = _fp4_matrix(w, "fp4_gemm")
+    if a.dim() != 2 or a.shape[1] != K or out.shape != (a.shape[0], N // 2 if silu_mul else N):
+        raise KernelError(f"fp4_gemm: shapes do not match: a {tuple(a.shape)}, w {(N, K)}, out {tuple(out.shape)}")
+    if silu_mul and (accumulate or N % 2):
+        raise KernelError("fp4_gemm: the fused SiLU-multiply takes an even number of rows of w and does not accumulate")
+    if accumulate and out.dtype != torch.float32:
+        raise KernelError("fp4_gemm: accumulation is into a 32-bit result")
+    _apart(a, out, "fp4_gemm: a and out share memory")
+    lda, ldo, dtype, out_dtype = _rows(a, "a"), _rows(out, "out"), dtype_code(a), dtype_code(out)
+    _here("fp4_gemm", a, *w, out, workspace)
+    lib = _lib("fp4_gemm")
+    _launch(lib, lib.gb_fp4_gemm, _p(a), dtype, lda, _p(w.codes), _p(w.scales), w.scales.shape[1], _p(out), out_dtype, ldo,
+            a.shape[0], N, K, 2 if silu_mul else 1 if accumulate else 0, _stream())
