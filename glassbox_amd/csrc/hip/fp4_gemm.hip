@@ -1,10 +1,18 @@
 // Products with four-bit weights (fp4.h): out (+)= a . W^T, or silu(a . gate^T) * (a . up^T) of a stack of both.
 //
-// Few rows: what bounds it is W's bytes, 17 / 32 of one a number.  W is the left operand of 16 x 16 x 32 products, so that a lane's
-// numbers are 32 neighbours of one row of W with one scale: 16 bytes and a byte.  They become bf16 in registers, two an instruction,
-// exactly, and never see LDS.  Waves of a workgroup take every W-th 128 numbers of k and are added up through LDS in their order.
-// The rows of a come from memory to every wave (they are in L2): NT tiles of 16 rows of W share what a wave reads of them.
-// 32-bit rows count as three bf16 terms (fp4.h): the products stay exact, their sums are in 32 bits either way.
+// W is the left operand of 16 x 16 x 32 products: a lane holds 32 neighbours of one row of W, a block: 16 bytes and a scale, which become
+// bf16 in registers, two numbers an instruction, exactly, and never see LDS.  32-bit rows count as three bf16 terms (fp4.h): the
+// products stay exact; all sums are in 32 bits.  Workgroups too few for the chip divide k into slices, which a second kernel adds up in
+// order (given a workspace).  Two kernels:
+//
+// lines (up to 16 rows): bound by W's bytes, 17 / 32 of one a number, and from a few rows on by what a compute unit brings in of a.  8 rows
+//   of W a tile, lanes r >= 8 with the same rows 128 numbers further on, so that a wave's load reads 8 whole lines of 128 bytes; the rows of
+//   a stand in the columns likewise, 8 of them, and of the 16 x 16 results the two quarters in which both are of one run of k are added up.
+//   The waves of a workgroup take turns over k and are joined through LDS.  (16 rows of W and half lines, us: 1 row by 128,256 of 4,096
+//   68.5, whole lines 55.8: 5.0 TB/s; 28,672 of 4,096 20.3 and 17.3; 2,048 of 8,192 7.1 and 5.4.)
+// tiles (more): a's rows go through LDS, 64 (32) of them by 128 or 256 rows of W, whose waves have rows of W of their own: 2,048 rows by
+//   28,672 of 4,096 in 534 us, 0.9 PFLOP/s; 64 rows in 36.  (Rows of a from memory to every wave: 60; what bounds it there is the way into a
+//   compute unit, 20 to 50 GB/s each.)
 #include "fp4.h"
 
 #include <algorithm>
@@ -15,99 +23,148 @@ struct GemmArgs {
   const void* x;
   const uint8_t *codes, *scales;
   void* out;
-  int ldx, ldo, M, N, blocks, scale_stride, n_tiles, m_tiles, epilogue, out32, x_wide;   // epilogue 0 store, 1 add, 2 silu(gate) * up
+  float* slices;   // [slices, M, N]: given, each slice of k leaves its sums there
+  int ldx, ldo, M, N, blocks, scale_stride, n_tiles, m_tiles, turns, epilogue, out32, out_wide;   // epilogue 0 store, 1 add, 2 silu(gate) * up
 };
 
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-__device__ __forceinline__ void put(const GemmArgs& a, int m, int n, int limit, const f32x4& v) {
+// four neighbouring columns of a row of out, those below `limit`
+__device__ __forceinline__ void put(const GemmArgs& a, int m, int n, int limit, f32x4 v) {
   const size_t at = (size_t)m * a.ldo + n;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (n + i < limit) {
-      if (a.out32) {
-        float* o = (float*)a.out + at + i;
-        *o = a.epilogue == 1 ? *o + v[i] : v[i];
-      } else {
-        ((bf16*)a.out)[at + i] = (bf16)v[i];
-      }
+  if (a.out32) {
+    float* o = (float*)a.out + at;
+    if (a.out_wide && n + 4 <= limit) {
+      if (a.epilogue == 1) v += *reinterpret_cast<const f32x4*>(o);
+      *reinterpret_cast<f32x4*>(o) = v;
+      return;
     }
+    for (int i = 0; i < 4 && n + i < limit; ++i) o[i] = a.epilogue == 1 ? o[i] + v[i] : v[i];
+  } else {
+    bf16* o = (bf16*)a.out + at;
+    if (a.out_wide && n + 4 <= limit) {
+      *reinterpret_cast<bf16x4*>(o) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+      return;
+    }
+    for (int i = 0; i < 4 && n + i < limit; ++i) o[i] = (bf16)v[i];
+  }
 }
 
-// T the rows' type, MT tiles of 16 rows of a, NT of 16 rows of W (with silu every other one of the up half), W waves
-template <typename T, int MT, int NT, int W>
-__global__ __launch_bounds__(W * kWave) void fp4_gemm_kernel(GemmArgs a) {
+// the same, or into the slice of k whose sum it is
+__device__ __forceinline__ void put_or_leave(const GemmArgs& a, int m, int n, int limit, f32x4 v) {
+  if (!a.slices) return put(a, m, n, limit, v);
+  float* o = a.slices + ((size_t)blockIdx.y * a.M + m) * a.N + n;
+  if (a.N % 4 == 0 && n + 4 <= limit) *reinterpret_cast<f32x4*>(o) = v;
+  else
+    for (int i = 0; i < 4 && n + i < limit; ++i) o[i] = v[i];
+}
+
+// eight elements of a row as they come from memory
+template <typename T> struct Raw {
+  u32x4 w[std::is_same_v<T, float> ? 2 : 1];
+};
+template <typename T> __device__ __forceinline__ void keep(Raw<T>& v, bool in) {   // zeros where not
+#pragma unroll
+  for (auto& w : v.w)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = in ? w[e] : 0u;
+}
+__device__ __forceinline__ void terms_of(const Raw<bf16>& v, bf16x8 (&out)[1]) { out[0] = __builtin_bit_cast(bf16x8, v.w[0]); }
+__device__ __forceinline__ void terms_of(const Raw<float>& v, bf16x8 (&out)[3]) {
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(v.w[e / 4][e % 4]);
+  fp4_terms<3>(x, out);
+}
+
+// T the rows' type, MT tiles of 8 rows of a, NT of 8 rows of W (with silu every other one of the up half), W waves, U blocks of 32 numbers of
+// k that a lane asks for at once
+template <typename T, int MT, int NT, int W, int U>
+__global__ __launch_bounds__(W * kWave) void fp4_lines_kernel(GemmArgs a) {
   constexpr int SP = kFp4Terms<T>;
   const int lane = threadIdx.x % kWave, r = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  // the row tiles of one tile of W follow each other on one XCD (workgroups go to the eight in turn), whose L2 then has it
-  const int turn = blockIdx.x / 8, nt = turn / a.m_tiles * 8 + blockIdx.x % 8, mt0 = turn % a.m_tiles * 16 * MT;
-  if (nt >= a.n_tiles) return;
+  const int nt = blockIdx.x;
   const bool silu = a.epilogue == 2;
   const int half = a.N / 2;
-  int row0[NT], limit[NT];
   const uint8_t *codes[NT], *scales[NT];
+  const T* x[MT];
+  auto row_of = [&](int p) { return silu ? (p & 1 ? half : 0) + (nt * (NT / 2) + p / 2) * 8 : (nt * NT + p) * 8; };
 #pragma unroll
   for (int p = 0; p < NT; ++p) {
-    row0[p] = silu ? (p & 1 ? half : 0) + (nt * (NT / 2) + p / 2) * 16 : (nt * NT + p) * 16;
-    limit[p] = silu && !(p & 1) ? half : a.N;
-    const int row = min(row0[p] + r, limit[p] - 1);
-    codes[p] = a.codes + (size_t)row * a.blocks * 16 + g * 16;
+    const int row = min(row_of(p) + r % 8, (silu && !(p & 1) ? half : a.N) - 1);
+    codes[p] = a.codes + (size_t)row * a.blocks * 16;
     scales[p] = a.scales + (size_t)row * a.scale_stride;
   }
-  const T* x[MT];
-  bool has[MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int m = mt0 + 16 * t + r;
-    has[t] = m < a.M;
-    x[t] = (const T*)a.x + (size_t)min(m, a.M - 1) * a.ldx + g * kFp4Block;
-  }
+  for (int t = 0; t < MT; ++t) x[t] = (const T*)a.x + (size_t)min(t * 8 + r % 8, a.M - 1) * a.ldx;
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int p = 0; p < NT; ++p)
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[p][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const int chunks = (a.blocks + 3) / 4;
-  u32x4 next[NT];
-  uint32_t nexts[NT];
-  auto fetch = [&](int c) {
-    const bool in = 4 * c + g < a.blocks;
+  // this lane's u-th block in turn i.  Loads do not branch: beyond the end they read the last block again
+  auto block = [&](int i, int u) { return 8 * ((i * W + wave) * U + u) + 4 * (r / 8) + g; };
+  u32x4 next[U][NT];
+  uint32_t next_scale[U][NT];
+  Raw<T> next_x[U][MT][4];
+  auto fetch = [&](int i) {
 #pragma unroll
-    for (int p = 0; p < NT; ++p) {
-      next[p] = in ? *reinterpret_cast<const u32x4*>(codes[p] + (size_t)c * 64) : u32x4{0, 0, 0, 0};
-      nexts[p] = *reinterpret_cast<const uint32_t*>(scales[p] + 4 * c);
-    }
-  };
-  if (wave < chunks) fetch(wave);
-  for (int c = wave; c < chunks; c += W) {
-    u32x4 now[NT];
-    float unit[NT];
-#pragma unroll
-    for (int p = 0; p < NT; ++p) now[p] = next[p], unit[p] = fp4_unit(nexts[p] >> (8 * g) & 255u);
-    const bool in = 4 * c + g < a.blocks;
-    bf16x8 xf[MT][4][SP];
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        float v[8] = {};
-        if (in && has[t]) load8(x[t] + (size_t)c * 128 + 8 * w, a.x_wide, v);
-        fp4_terms<SP>(v, xf[t][w]);
-      }
-    if (c + W < chunks) fetch(c + W);
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
+    for (int u = 0; u < U; ++u) {
+      const int c = min(block(i, u), a.blocks - 1);
 #pragma unroll
       for (int p = 0; p < NT; ++p) {
-        const bf16x8 kf = fp4_unpack8(now[p][w], unit[p]);
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int q = 0; q < SP; ++q) acc[p][t] = mfma(kf, xf[t][w][q], acc[p][t]);
+        next[u][p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(codes[p] + (size_t)c * 16));
+        next_scale[u][p] = scales[p][c];
       }
-  }
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)   // (rows may begin anywhere: the hardware takes 16 bytes from any address)
+          __builtin_memcpy(&next_x[u][t][w], x[t] + (size_t)c * kFp4Block + 8 * w, sizeof(Raw<T>));
+    }
+  };
+  const int first = blockIdx.y * a.turns, turns = (a.blocks + 8 * U * W - 1) / (8 * U * W), end = min(turns, first + a.turns);
+  // (the last turn stands by itself: a load behind a branch would be waited for together with all others)
+  auto turn = [&](int i, auto last) {
+    u32x4 now[U][NT];
+    float unit[U][NT];
+    Raw<T> raw[U][MT][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = !last || block(i, u) < a.blocks;   // what is beyond the end counts as zero
+#pragma unroll
+      for (int p = 0; p < NT; ++p) now[u][p] = next[u][p], unit[u][p] = in ? fp4_unit(next_scale[u][p]) : 0.f;
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          raw[u][t][w] = next_x[u][t][w];
+          if constexpr (last) keep(raw[u][t][w], in);
+        }
+    }
+    if constexpr (!last) fetch(i + 1);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        bf16x8 xf[MT][SP];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) terms_of(raw[u][t][w], xf[t]);
+#pragma unroll
+        for (int p = 0; p < NT; ++p) {
+          const bf16x8 kf = fp4_unpack8(now[u][p][w], unit[u][p]);
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int q = 0; q < SP; ++q) acc[p][t] = mfma(kf, xf[t][q], acc[p][t]);
+        }
+      }
+  };
+  fetch(first);
+  for (int i = first; i + 1 < end; ++i) turn(i, std::false_type{});
+  turn(end - 1, std::true_type{});
 
   __shared__ f32x4 part[W][NT * MT][kWave];
 #pragma unroll
@@ -115,50 +172,241 @@ __global__ __launch_bounds__(W * kWave) void fp4_gemm_kernel(GemmArgs a) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) part[wave][p * MT + t][lane] = acc[p][t];
   __syncthreads();
+  // lane (r, g) of a tile's total: rows 4 g .. of W, row r of a; the quarters g < 2, r < 8 and g >= 2, r >= 8 are of two runs of k
   auto total = [&](int tile) {
-    f32x4 v = part[0][tile][lane];
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 1; w < W; ++w) v += part[w][tile][lane];
+    for (int w = 0; w < W; ++w) v += part[w][tile][lane] + part[w][tile][lane ^ 40];
     return v;
   };
-  if (silu) {
+  if (silu && !a.slices) {
     for (int u = wave; u < NT / 2 * MT; u += W) {
-      const int p = u / MT * 2, t = u % MT, m = mt0 + 16 * t + r;
+      const int p = u / MT * 2, t = u % MT, m = 8 * t + r;
       const f32x4 gate = total(p * MT + t), up = total((p + 1) * MT + t);
       f32x4 v;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = silu_times(gate[i], up[i]);
-      if (m < a.M) put(a, m, (nt * (NT / 2) + p / 2) * 16 + 4 * g, half, v);
+      if (m < a.M && r < 8 && g < 2) put(a, m, row_of(p) + 4 * g, half, v);
     }
   } else {
     for (int u = wave; u < NT * MT; u += W) {
-      const int p = u / MT, t = u % MT, m = mt0 + 16 * t + r;
+      const int p = u / MT, t = u % MT, m = 8 * t + r;
       const f32x4 v = total(u);
-      if (m < a.M) put(a, m, (nt * NT + p) * 16 + 4 * g, a.N, v);
+      if (m < a.M && r < 8 && g < 2) put_or_leave(a, m, row_of(p) + 4 * g, silu && !(p & 1) ? half : a.N, v);
     }
   }
 }
 
-template <typename T, int MT, int NT, int W> static void launch(GemmArgs a, hipStream_t stream) {
-  const int rows = a.epilogue == 2 ? a.N / 2 : a.N, per = 16 * (a.epilogue == 2 ? NT / 2 : NT);
-  a.n_tiles = (rows + per - 1) / per;
-  a.m_tiles = (a.M + 16 * MT - 1) / (16 * MT);
-  hipLaunchKernelGGL((fp4_gemm_kernel<T, MT, NT, W>), dim3((unsigned)((a.n_tiles + 7) / 8 * 8 * a.m_tiles)), dim3(W * kWave), 0, stream, a);
+// T the rows' type, MT tiles of 16 rows of a (all waves'), NT of 16 rows of W a wave, B blocks of 32 numbers of k a step.  a's rows pass
+// through LDS, a step ahead in registers, the words of a row exchanged by the row so that the operands' reads spread over the banks.
+template <typename T, int MT, int NT, int B>
+__global__ __launch_bounds__(256) void fp4_tiles_kernel(GemmArgs a) {
+  constexpr int SP = kFp4Terms<T>, W = 4, U = B / 4, kRows = 16 * MT, kWords = 4 * B, kLoads = kRows * kWords / 256, kStep = 256 / kWords;
+  __shared__ bf16x8 xs[2][SP][kRows * kWords];
+  const int lane = threadIdx.x % kWave, r = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  // the row tiles of one tile of W follow each other on one XCD (workgroups go to the eight in turn), whose L2 then has it
+  const int order = blockIdx.x / 8, nt = order / a.m_tiles * 8 + blockIdx.x % 8, mt0 = order % a.m_tiles * kRows;
+  if (nt >= a.n_tiles) return;
+  const bool silu = a.epilogue == 2;
+  const int half = a.N / 2;
+  const uint8_t *codes[NT], *scales[NT];
+  auto row_of = [&](int p) {
+    const int i = (nt * W + wave) * NT + p;
+    return silu ? (i & 1 ? half : 0) + i / 2 * 16 : i * 16;
+  };
+#pragma unroll
+  for (int p = 0; p < NT; ++p) {
+    const int row = min(row_of(p) + r, (silu && !(p & 1) ? half : a.N) - 1);
+    codes[p] = a.codes + (size_t)row * a.blocks * 16;
+    scales[p] = a.scales + (size_t)row * a.scale_stride;
+  }
+  const int word = threadIdx.x % kWords, row0 = threadIdx.x / kWords;   // what this thread brings of a: eight numbers of every kStep-th row
+  const T* x[kLoads];
+#pragma unroll
+  for (int l = 0; l < kLoads; ++l) x[l] = (const T*)a.x + (size_t)min(mt0 + row0 + l * kStep, a.M - 1) * a.ldx;
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int p = 0; p < NT; ++p)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[p][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  u32x4 next[U][NT];
+  uint32_t next_scale[U][NT];
+  Raw<T> next_x[kLoads];
+  auto fetch = [&](int i) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = min(i * B + U * g + u, a.blocks - 1);
+#pragma unroll
+      for (int p = 0; p < NT; ++p) {
+        next[u][p] = *reinterpret_cast<const u32x4*>(codes[p] + (size_t)c * 16);
+        next_scale[u][p] = scales[p][c];
+      }
+    }
+    const int c = min(i * B + word / 4, a.blocks - 1);
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) __builtin_memcpy(&next_x[l], x[l] + (size_t)c * kFp4Block + word % 4 * 8, sizeof(Raw<T>));
+  };
+  auto bring = [&](int i, int buffer) {
+    const bool in = i * B + word / 4 < a.blocks;
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) {
+      const int row = row0 + l * kStep;
+      Raw<T> v = next_x[l];
+      keep(v, in);
+      bf16x8 terms[SP];
+      terms_of(v, terms);
+#pragma unroll
+      for (int q = 0; q < SP; ++q) xs[buffer][q][row * kWords + (word ^ (row & 15))] = terms[q];
+    }
+  };
+  const int first = blockIdx.y * a.turns, turns = (a.blocks + B - 1) / B, end = min(turns, first + a.turns);
+  auto turn = [&](int i, int buffer, auto last) {
+    u32x4 now[U][NT];
+    float unit[U][NT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = i * B + U * g + u < a.blocks;
+#pragma unroll
+      for (int p = 0; p < NT; ++p) now[u][p] = next[u][p], unit[u][p] = in ? fp4_unit(next_scale[u][p]) : 0.f;
+    }
+    if constexpr (!last) fetch(i + 1);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        bf16x8 kf[NT];
+#pragma unroll
+        for (int p = 0; p < NT; ++p) kf[p] = fp4_unpack8(now[u][p][w], unit[u][p]);
+#pragma unroll
+        for (int q = 0; q < SP; ++q) {
+          bf16x8 xf[MT];
+#pragma unroll
+          for (int t = 0; t < MT; ++t) xf[t] = xs[buffer][q][(16 * t + r) * kWords + (((U * g + u) * 4 + w) ^ r)];
+#pragma unroll
+          for (int p = 0; p < NT; ++p)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[p][t] = mfma(kf[p], xf[t], acc[p][t]);
+        }
+      }
+    if constexpr (!last) {   // into the half that was read a turn ago: every wave has passed the barrier behind that
+      bring(i + 1, buffer ^ 1);
+      __syncthreads();
+    }
+  };
+  fetch(first);
+  bring(first, 0);
+  __syncthreads();
+  int buffer = 0;
+  for (int i = first; i + 1 < end; ++i, buffer ^= 1) turn(i, buffer, std::false_type{});
+  turn(end - 1, buffer, std::true_type{});
+
+  // lane (r, g): row r of a tile of a, rows 4 g .. of W
+#pragma unroll
+  for (int p = 0; p < NT; ++p) {
+    const int n = row_of(p) + 4 * g;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const int m = mt0 + 16 * t + r;
+      if (m >= a.M) continue;
+      if (!silu || a.slices) {
+        put_or_leave(a, m, n, silu && !(p & 1) ? half : a.N, acc[p][t]);
+      } else if (p & 1) {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = silu_times(acc[p - 1][t][e], acc[p][t][e]);
+        put(a, m, n - half, half, v);
+      }
+    }
+  }
 }
 
-template <typename T> static void launch_by(const GemmArgs& a, hipStream_t stream) {
-  const int tiles = (a.N + 15) / 16;
-  const bool silu = a.epilogue == 2;
-  if (a.M <= 16) {
-    if (tiles >= 2048) launch<T, 1, 4, 4>(a, stream);
-    else if (silu || tiles >= 512) launch<T, 1, 2, 8>(a, stream);
-    else launch<T, 1, 1, 8>(a, stream);
-  } else if (a.M <= 32) {
-    if (tiles >= 1024) launch<T, 2, 4, 4>(a, stream);
-    else launch<T, 2, 2, 4>(a, stream);
-  } else {
-    if (tiles >= 1024 || a.M > 128) launch<T, 4, 4, 4>(a, stream);
-    else launch<T, 4, 2, 4>(a, stream);
+// Adds up the slices of k, in their order, and does what the epilogue does.  A thread a column (of both halves, with silu).
+__global__ __launch_bounds__(256) void fp4_gemm_join_kernel(GemmArgs a, int slices) {
+  const int cols = a.epilogue == 2 ? a.N / 2 : a.N;
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int m = (int)(at / cols), n = (int)(at % cols);
+  if (m >= a.M) return;
+  const size_t step = (size_t)a.M * a.N;
+  const float* p = a.slices + (size_t)m * a.N + n;
+  float v = 0.f, u = 0.f;
+#pragma unroll 8
+  for (int z = 0; z < slices; ++z) {
+    v += p[z * step];
+    if (a.epilogue == 2) u += p[z * step + cols];
+  }
+  if (a.epilogue == 2) v = silu_times(v, u);
+  const size_t o = (size_t)m * a.ldo + n;
+  if (!a.out32) ((bf16*)a.out)[o] = (bf16)v;
+  else if (a.epilogue == 1) ((float*)a.out)[o] += v;
+  else ((float*)a.out)[o] = v;
+}
+
+// Which kernel takes a product, and how: a function of its sizes and type alone.
+struct Form {
+  int rows_w, rows_a, step;   // a workgroup's rows of W and of a, blocks of k a turn
+};
+// lines: MT x NT, waves (a turn is 8 U blocks a wave)      1 x 4, 8       1 x 2, 8       1 x 1, 8 (U 2)   2 x 8, 4        2 x 4, 8
+// tiles: MT x NT, blocks                                   2 x 2, 8       4 x 2, 8       4 x 4, 4         2 x 2, 4 and 4 x 2, 4 (32-bit rows)
+static constexpr Form kForms[] = {{32, 8, 64}, {16, 8, 64}, {8, 8, 128}, {64, 16, 32}, {32, 16, 64}, {128, 32, 8}, {128, 64, 8}, {256, 64, 4},
+                                  {128, 32, 4}, {128, 64, 4}};
+struct Plan {
+  int form, n_tiles, m_tiles, turns, slices;
+};
+
+static Plan plan(int M, int N, int K, bool silu, int dtype) {
+  auto tiles = [&](int form) { return (long long)((N + kForms[form].rows_w - 1) / kForms[form].rows_w) * ((M + kForms[form].rows_a - 1) / kForms[form].rows_a); };
+  Plan p;
+  // up to 8 rows: as many rows of W a workgroup as leave about 192 of them (16 with silu, which takes pairs of tiles).  us, 8 rows: 6,144 of
+  // 4,096 by 32 7.8, by 16 8.5; 4,096 of 14,336 by 16 14.1, by 32 21; 2,048 of 8,192 by 8 8.1, by 16 11.
+  if (M <= 8) p.form = N >= 6144 ? 0 : N >= 4096 || silu ? 1 : 2;
+  // up to 16: 28,672 of 4,096 by 64 24.2, by 32 29; 6,144 of 4,096 by 32 9.8, by 64 14
+  else if (M <= 16) p.form = N >= 16384 ? 3 : 4;
+  // more: 64 x 256 where there are enough of them: 256 rows by 28,672 of 4,096 82 (64 x 128 87), by 4,096 of 4,096 27 (24.5)
+  else if (dtype == kF32) p.form = M <= 32 ? 8 : 9;
+  else p.form = M <= 32 ? 5 : tiles(7) >= 384 ? 7 : 6;
+  const Form f = kForms[p.form];
+  p.n_tiles = silu ? (N / 2 + f.rows_w / 2 - 1) / (f.rows_w / 2) : (N + f.rows_w - 1) / f.rows_w;
+  p.m_tiles = (M + f.rows_a - 1) / f.rows_a;
+  const int turns = (K / 32 + f.step - 1) / f.step;
+  // slices of k, us: 16 rows by 4,096 of 14,336 in 2 18.3 (1: 29); 32 in 8 19.9 (1: 41); 128 in 8 33.1; 64 by 4,096 of 4,096 in 8 15.9 (1: 21)
+  const long long groups = (long long)p.n_tiles * p.m_tiles;
+  const long long want = M <= 8 ? 1 : M <= 16 ? 256 / groups : groups <= 224 ? (384 + groups - 1) / groups : 1;
+  const int slices = (int)std::max<long long>(1, std::min<long long>(want, turns));
+  p.turns = (turns + slices - 1) / slices;
+  p.slices = (turns + p.turns - 1) / p.turns;
+  return p;
+}
+
+template <typename T, int MT, int NT, int W, int U> static void lines(const Plan& p, const GemmArgs& a, hipStream_t stream) {
+  static_assert(MT * NT * W <= 64, "the waves' sums fill LDS");
+  hipLaunchKernelGGL((fp4_lines_kernel<T, MT, NT, W, U>), dim3((unsigned)p.n_tiles, (unsigned)p.slices), dim3(W * kWave), 0, stream, a);
+}
+template <typename T, int MT, int NT, int B> static void tiles(const Plan& p, const GemmArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((fp4_tiles_kernel<T, MT, NT, B>), dim3((unsigned)((p.n_tiles + 7) / 8 * 8 * p.m_tiles), (unsigned)p.slices), dim3(256), 0, stream, a);
+}
+
+template <typename T> static void launch_by(const Plan& p, const GemmArgs& a, hipStream_t stream) {
+  switch (p.form) {
+    case 0: lines<T, 1, 4, 8, 1>(p, a, stream); break;
+    case 1: lines<T, 1, 2, 8, 1>(p, a, stream); break;
+    case 2: lines<T, 1, 1, 8, 2>(p, a, stream); break;
+    case 3: lines<T, 2, 8, 4, 1>(p, a, stream); break;
+    case 4: lines<T, 2, 4, 8, 1>(p, a, stream); break;
+    default:
+      if constexpr (std::is_same_v<T, float>) {
+        if (p.form == 8) tiles<T, 2, 2, 4>(p, a, stream);
+        else tiles<T, 4, 2, 4>(p, a, stream);
+      } else {
+        if (p.form == 5) tiles<T, 2, 2, 8>(p, a, stream);
+        else if (p.form == 6) tiles<T, 4, 2, 8>(p, a, stream);
+        else tiles<T, 4, 4, 4>(p, a, stream);
+      }
+  }
+  if (p.slices > 1) {
+    const long long cells = (long long)a.M * (a.epilogue == 2 ? a.N / 2 : a.N);
+    hipLaunchKernelGGL(fp4_gemm_join_kernel, dim3((unsigned)((cells + 255) / 256)), dim3(256), 0, stream, a, p.slices);
   }
 }
 
@@ -166,8 +414,15 @@ template <typename T> static void launch_by(const GemmArgs& a, hipStream_t strea
 
 using namespace gb;
 
+// floats of workspace with which k is divided; 0: it is not
+extern "C" long long gb_fp4_gemm_floats(int M, int N, int K, int epilogue, int dtype) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const Plan p = plan(M, N, K, epilogue == 2, dtype);
+  return p.slices > 1 ? (long long)p.slices * M * N : 0;
+}
+
 extern "C" int gb_fp4_gemm(const void* x, int dtype, int ldx, const void* codes, const void* scales, int scale_stride, void* out, int out_dtype,
-                           int ldo, int M, int N, int K, int epilogue, hipStream_t stream) {
+                           int ldo, int M, int N, int K, int epilogue, float* workspace, long long workspace_floats, hipStream_t stream) {
   GB_REQUIRE(M >= 0 && N > 0 && K > 0 && K % 32 == 0, "fp4_gemm: bad sizes M=%d N=%d K=%d", M, N, K);
   GB_REQUIRE(epilogue >= 0 && epilogue <= 2 && (epilogue != 2 || N % 2 == 0), "fp4_gemm: epilogue %d of %d columns", epilogue, N);
   GB_REQUIRE(epilogue != 1 || out_dtype == kF32, "fp4_gemm: accumulation is into a 32-bit result");
@@ -176,12 +431,17 @@ extern "C" int gb_fp4_gemm(const void* x, int dtype, int ldx, const void* codes,
              "fp4_gemm: codes and scales begin at 16-byte words, rows of scales are multiples of 16");
   GB_REQUIRE((dtype == kF32 || dtype == kBF16) && (out_dtype == kF32 || out_dtype == kBF16), "fp4_gemm: unknown dtype %d or %d", dtype, out_dtype);
   if (M == 0) return 0;
-  GB_REQUIRE((long long)((N + 15) / 16 + 8) * ((M + 15) / 16) < (1ll << 31), "fp4_gemm: %d x %d is too much for one launch", M, N);
-  const int e = dtype == kF32 ? 4 : 2;
-  GemmArgs a{x, (const uint8_t*)codes, (const uint8_t*)scales, out, ldx, ldo, M, N, K / 32, scale_stride, 0, 0, epilogue, out_dtype == kF32,
-             ((uintptr_t)x & 15) == 0 && (size_t)ldx * e % 16 == 0};
-  if (dtype == kF32) launch_by<float>(a, stream);
-  else launch_by<bf16>(a, stream);
+  Plan p = plan(M, N, K, epilogue == 2, dtype);
+  if (p.slices > 1 && (!workspace || workspace_floats < (long long)p.slices * M * N)) {   // whole k a workgroup: slower, not refused
+    p.turns *= p.slices;
+    p.slices = 1;
+  }
+  GB_REQUIRE((long long)(p.n_tiles + 7) * p.m_tiles < (1ll << 31) && (long long)M * N < (1ll << 38), "fp4_gemm: %d x %d is too much for one launch", M, N);
+  const int e = out_dtype == kF32 ? 16 : 8;   // bytes of four columns
+  const GemmArgs a{x, (const uint8_t*)codes, (const uint8_t*)scales, out, p.slices > 1 ? workspace : nullptr, ldx, ldo, M, N, K / 32, scale_stride,
+                   p.n_tiles, p.m_tiles, p.turns, epilogue, out_dtype == kF32, (uintptr_t)out % e == 0 && ldo % 4 == 0};
+  if (dtype == kF32) launch_by<float>(p, a, stream);
+  else launch_by<bf16>(p, a, stream);
   return launched("fp4_gemm");
 }
 

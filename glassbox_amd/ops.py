@@ -290,8 +290,9 @@ _SIGS = {
         "gb_fp4_attention_takes": [_i],
     },
     "fp4_gemm": {
-        # a, dtype, lda, codes, scales, scales a row, out, its dtype, ldo, M, N, K, epilogue, stream
-        "gb_fp4_gemm": [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp],
+        # a, dtype, lda, codes, scales, scales a row, out, its dtype, ldo, M, N, K, epilogue, workspace, its floats, stream
+        "gb_fp4_gemm": [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, C.c_longlong, _vp],
+        "gb_fp4_gemm_floats": [_i, _i, _i, _i, _i],
     },
     "sampling": {
         "gb_argmax": [_vp, _vp, _i, _i, _vp],
@@ -2767,16 +2768,31 @@ def fp4_expand(w: Fp4Matrix, out: torch.Tensor) -> None:
     _launch(lib, lib.gb_fp4_expand, _p(w.codes), _p(w.scales), _p(out), dtype, n, k, w.scales.shape[1], _stream())
 
 
-def fp4_gemm_floats(rows: int, n: int, k: int, dtype: torch.dtype = torch.bfloat16) -> int:
-    """Floats of workspace with which ``fp4_gemm`` is faster for so many rows; 0 if it has no use for any."""
-    return 0
+def _fp4_expands(rows: int, n: int, k: int, dtype: torch.dtype, out_dtype: torch.dtype, silu_mul: bool) -> bool:
+    """Whether a product goes through the weights' bfloat16 values, given the workspace for them: ``gemm`` takes many rows in fewer us than the
+    kernel that converts on the way, and more than the values cost: 2,048 rows by 28,672 of 4,096 59 + 417 us and 534, by 4,096 of 4,096 8.5
+    + 75.5 and 80."""
+    return (rows >= 1536 and n * k >= 1 << 26 and dtype == torch.bfloat16 and not (silu_mul and (n % 16 or out_dtype != torch.bfloat16)))
+
+
+@functools.lru_cache(maxsize=4096)   # a pure function of the sizes, asked for at every product
+def fp4_gemm_floats(rows: int, n: int, k: int, dtype: torch.dtype = torch.bfloat16, out_dtype: Optional[torch.dtype] = None,
+                    silu_mul: bool = False) -> int:
+    """Floats of workspace with which ``fp4_gemm`` takes ``rows`` rows by ``n`` rows of w of ``k`` numbers faster; 0 if it has no use for any."""
+    if _fp4_expands(rows, n, k, dtype, out_dtype or dtype, silu_mul):
+        return n * k // 2 + gemm_split_floats(rows, n, k)
+    f = _lib("fp4_gemm").gb_fp4_gemm_floats
+    f.restype = C.c_longlong
+    return int(f(int(rows), int(n), int(k), 2 if silu_mul else 0, F32 if dtype == torch.float32 else BF16))
 
 
 def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool = False, silu_mul: bool = False,
              workspace: Optional[torch.Tensor] = None) -> None:
     """out (+)= a . w^T with four-bit weights, the sums in 32 bits: ``a`` [rows, columns of w] bfloat16 or float32, ``out`` bfloat16 or float32
     (float32 when accumulating).  ``silu_mul``: w stacks gate rows over up rows and out[m, j] = silu(a . gate_j) * (a . up_j), of half as
-    many columns.  ``workspace`` (float32, ``fp4_gemm_floats`` elements) is optional."""
+    many columns.
+    ``workspace`` (float32, ``fp4_gemm_floats`` elements; optional): lets few workgroups divide k (their sums are added in a fixed order), and
+    large bfloat16 products have the weights' bfloat16 values written there first and multiplied by ``gemm``."""
     N, K = _fp4_matrix(w, "fp4_gemm")
     if a.dim() != 2 or a.shape[1] != K or out.shape != (a.shape[0], N // 2 if silu_mul else N):
         raise KernelError(f"fp4_gemm: shapes do not match: a {tuple(a.shape)}, w {(N, K)}, out {tuple(out.shape)}")
@@ -2785,8 +2801,17 @@ def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool 
     if accumulate and out.dtype != torch.float32:
         raise KernelError("fp4_gemm: accumulation is into a 32-bit result")
     _apart(a, out, "fp4_gemm: a and out share memory")
+    if workspace is not None and (workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.data_ptr() % 16):
+        raise KernelError("fp4_gemm: the workspace must be contiguous float32 that begins at a 16-byte word")
     lda, ldo, dtype, out_dtype = _rows(a, "a"), _rows(out, "out"), dtype_code(a), dtype_code(out)
     _here("fp4_gemm", a, *w, out, workspace)
+    M, floats = a.shape[0], workspace.numel() if workspace is not None else 0
+    if floats >= N * K // 2 and _fp4_expands(M, N, K, a.dtype, out.dtype, silu_mul) and lda % 8 == 0 and a.data_ptr() % 16 == 0:
+        values = workspace[:N * K // 2].view(torch.bfloat16).view(N, K)
+        rest = workspace[N * K // 2:]
+        fp4_expand(w, values)
+        gemm(a, values, out, accumulate=accumulate, silu_mul=silu_mul, workspace=rest if rest.numel() >= max(1, gemm_split_floats(M, N, K)) else None)
+        return
     lib = _lib("fp4_gemm")
-    _launch(lib, lib.gb_fp4_gemm, _p(a), dtype, lda, _p(w.codes), _p(w.scales), w.scales.shape[1], _p(out), out_dtype, ldo,
-            a.shape[0], N, K, 2 if silu_mul else 1 if accumulate else 0, _stream())
+    _launch(lib, lib.gb_fp4_gemm, _p(a), dtype, lda, _p(w.codes), _p(w.scales), w.scales.shape[1], _p(out), out_dtype, ldo, M, N, K,
+            2 if silu_mul else 1 if accumulate else 0, _p(workspace), floats, _stream())

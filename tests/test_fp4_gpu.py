@@ -327,7 +327,7 @@ def test_attention_and_store_reach_pages_beyond_four_gigabytes():
 
 # ------------------------------------------------------------------------------------------------------------------- products
 GEMMS = [(1, 1, 32), (1, 40, 64), (3, 17, 96), (16, 64, 512), (17, 130, 544), (5, 2563, 992), (33, 300, 2048), (64, 96, 4128), (65, 48, 160),
-         (130, 1040, 256), (1, 8200, 1056), (2, 33000, 128), (20, 16500, 160), (300, 70, 992)]
+         (130, 1040, 256), (16, 17000, 96), (9, 520, 4128), (1, 8200, 1056), (2, 33000, 128), (20, 16500, 160), (300, 70, 992)]
 
 
 @pytest.mark.parametrize("M,N,K", GEMMS)
@@ -363,13 +363,35 @@ def test_gemm(M, N, K, dtype, out_dtype, how):
         mine = out[:, odd:odd + cols]
         if how == "add":
             mine.copy_(first)
-        floats = ops.fp4_gemm_floats(M, N, K, dtype)
+        floats = ops.fp4_gemm_floats(M, N, K, dtype, out_dtype, how == "silu")
         ops.fp4_gemm(given, w, mine, accumulate=how == "add", silu_mul=how == "silu",
                      workspace=torch.full((floats,), math.nan, device=DEV) if floats else None)
         far = (mine.double() - y).abs() > off
         assert not far.any(), (float((mine.double() - y).abs()[far].max()), float(off[far].max()))
         if odd:
             assert (out[:, :odd] == 3).all() and (out[:, odd + cols:] == 3).all()
+
+
+@pytest.mark.parametrize("M,N,K,how", [(1540, 8208, 8192, "silu"), (1600, 8200, 8192, "add"), (700, 8300, 640, "store"), (260, 28672, 96, "silu")])
+def test_gemm_of_many_rows(M, N, K, how):
+    """Through the weights' values and in tiles, with the workspace and without it: of one size within rounding."""
+    from glassbox_amd import ops
+    w = ops.fp4_quantize((torch.randn(N, K, generator=torch.Generator().manual_seed(27)) * 0.05).to(DEV))
+    wd = torch.empty(N, K, device=DEV)
+    ops.fp4_expand(w, wd)
+    a = normal(M, K, seed=28).bfloat16().to(DEV)
+    out_dtype, cols = (torch.float32, N) if how == "add" else (torch.bfloat16, N // 2 if how == "silu" else N)
+    y, size = a.double() @ wd.double().t(), a.double().abs() @ wd.double().abs().t()
+    off = (3 * K + 16) * STEP * size
+    if how == "silu":
+        g, u, dg, du = y[:, :cols], y[:, cols:], off[:, :cols], off[:, cols:]
+        y, off = g * torch.sigmoid(g) * u, 1.1 * dg * (u.abs() + du) + (g.abs() + dg) * du + 8 * STEP * (g * u).abs()
+    off = off + half_step(out_dtype) * (y.abs() + off) + 1e-30
+    floats = ops.fp4_gemm_floats(M, N, K, torch.bfloat16, out_dtype, how == "silu")
+    for ws in ([None] if floats == 0 else [None, torch.full((floats,), math.nan, device=DEV)]):
+        out = torch.zeros(M, cols, dtype=out_dtype, device=DEV)
+        ops.fp4_gemm(a, w, out, accumulate=how == "add", silu_mul=how == "silu", workspace=ws)
+        assert ((out.double() - y).abs() <= off).all()
 
 
 def test_gemm_of_rows_and_weights_that_are_not_finite():
