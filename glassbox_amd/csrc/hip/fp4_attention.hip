@@ -83,9 +83,10 @@ template <typename T> __device__ __forceinline__ void store4(T* p, bool wide, co
   for (int i = 0; i < 4; ++i) p[i] = (T)x[i];
 }
 
-// T the rows' type, NB blocks a head, R column tiles a wave, W waves, COLS: the waves have columns of their own
+// T the rows' type, NB blocks a head, R column tiles a wave, W waves, COLS: the waves have columns of their own.  (Two waves a SIMD at least
+// where they do: without the bound 2,048 rows of 32 heads of 128 take 108 us, with it 84.)
 template <typename T, int NB, int R, int W, bool COLS>
-__global__ __launch_bounds__(W * kWave) void fp4_attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(COLS && NB <= 4 ? 2 : 1))) void fp4_attend_kernel(AttendArgs a) {
   using U = Units<NB>;
   constexpr int D = NB * kFp4Block, SP = kFp4Terms<T>, C = 16 * R;
   static_assert(COLS || R == 1, "waves that share their columns hold one tile of them");
@@ -109,6 +110,22 @@ __global__ __launch_bounds__(W * kWave) void fp4_attend_kernel(AttendArgs a) {
   const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
   const int begin = (lo & ~(kTile - 1)) + split * a.chunk;
   const int end = min(min(last + 1, a.table_cols * a.page), begin + a.chunk);
+
+  // The numbers of a tile's pages are asked for a tile ahead, those of the first before the queries.  What is no page of the pool is not
+  // read (page 0 is, in its place), its keys are not seen.
+  const int32_t* table = a.tables + (size_t)s * a.table_stride;
+  const int start = begin + (COLS ? 0 : wave * kTile), stride = COLS ? kTile : W * kTile;
+  int kp, vp, koff, voff;   // of this lane's keys, 16 tokens all of which one page holds, and of its values
+  auto look_up = [&](int t0) {
+    const int kt = t0 + 16 * (r >> 2), vt = t0 + 16 * g;
+    const int ki = a.page_shift >= 0 ? kt >> a.page_shift : kt / a.page, vi = a.page_shift >= 0 ? vt >> a.page_shift : vt / a.page;
+    koff = kt - ki * a.page;
+    voff = vt - vi * a.page;
+    const int k0 = table[min(ki, a.table_cols - 1)], v0 = table[min(vi, a.table_cols - 1)];
+    kp = ki < a.table_cols ? k0 : -1;
+    vp = vi < a.table_cols ? v0 : -1;
+  };
+  look_up(start);
 
   int pos[R], from[R];   // a column sees the keys from .. pos
   bool own[R];
@@ -145,19 +162,12 @@ __global__ __launch_bounds__(W * kWave) void fp4_attend_kernel(AttendArgs a) {
   }
 
   const size_t block = fp4_block_bytes(a.page), head_bytes = block * NB;
-  const int32_t* table = a.tables + (size_t)s * a.table_stride;
   const int kslot = r & 3;
-  for (int t0 = begin + (COLS ? 0 : wave * kTile); t0 < end; t0 += COLS ? kTile : W * kTile) {
-    // the pages of this lane's keys and of its values; what is no page of the pool is not read, its keys are not seen
-    const int kt = t0 + 16 * (r >> 2), vt = t0 + 16 * g;
-    const int ki = a.page_shift >= 0 ? kt >> a.page_shift : kt / a.page, vi = a.page_shift >= 0 ? vt >> a.page_shift : vt / a.page;
-    int kp = ki < a.table_cols ? table[ki] : -1, vp = vi < a.table_cols ? table[vi] : -1;
+  for (int t0 = start; t0 < end; t0 += stride) {
+    const int vt = t0 + 16 * g;
     const bool known = (unsigned)vp < (unsigned)a.pages;
-    kp = (unsigned)kp < (unsigned)a.pages ? kp : 0;
-    vp = known ? vp : 0;
-    const int koff = kt - ki * a.page, voff = vt - vi * a.page;
-    const uint8_t* kb = a.k + ((size_t)kp * a.nkv + kvh) * head_bytes;
-    const uint8_t* vb = a.v + ((size_t)vp * a.nkv + kvh) * head_bytes;
+    const uint8_t* kb = a.k + ((size_t)((unsigned)kp < (unsigned)a.pages ? kp : 0) * a.nkv + kvh) * head_bytes;
+    const uint8_t* vb = a.v + ((size_t)(known ? vp : 0) * a.nkv + kvh) * head_bytes;
 
     uint32_t kw[4][NB], ks[U::kCount];
     u32x4 vw[NB], vs[NB];
@@ -186,6 +196,7 @@ __global__ __launch_bounds__(W * kWave) void fp4_attend_kernel(AttendArgs a) {
       vw[b] = *reinterpret_cast<const u32x4*>(vb + (size_t)b * block + (size_t)r * a.page + voff);
       vs[b] = *reinterpret_cast<const u32x4*>(vb + (size_t)b * block + (size_t)16 * a.page + voff);
     }
+    look_up(t0 + stride);
 
     f32x4 sc[R][4];
 #pragma unroll
@@ -395,8 +406,7 @@ __global__ __launch_bounds__(W * kWave) void fp4_attend_kernel(AttendArgs a) {
     for (int e = 0; e < kEach; ++e) {
       x[e] = 0.f;
 #pragma unroll
-      for (int w = 0; w < W; ++w)
-        if (weight[w] > 0.f) x[e] = fmaf(weight[w], so[w][column][part * kEach + e], x[e]);
+      for (int w = 0; w < W; ++w) x[e] = fmaf(weight[w], so[w][column][part * kEach + e], x[e]);
     }
     if (a.splits > 1) {
       const size_t at = (column0 + c) * a.splits + split;
@@ -426,13 +436,12 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int columns
   const float sum = wave_sum(weight * ml.y), over = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   constexpr int kEach = (D + kWave - 1) / kWave;
   float x[kEach] = {};
+  // (runs in which a column sees nothing have left zeros)
+#pragma unroll 8
   for (int i = 0; i < a.splits; ++i) {
     const float w = __shfl(weight, i, kWave);
-    if (w > 0.f) {
 #pragma unroll
-      for (int e = 0; e < kEach; ++e)
-        if (lane + e * kWave < D) x[e] = fmaf(w, a.acc[((size_t)at * a.splits + i) * D + lane + e * kWave], x[e]);
-    }
+    for (int e = 0; e < kEach; ++e) x[e] = fmaf(w, a.acc[((size_t)at * a.splits + i) * D + min(lane + e * kWave, D - 1)], x[e]);
   }
   T* row = (T*)a.out + (size_t)(q_start + token) * a.out_stride + (size_t)(kvh * a.rep + c % a.rep) * D;
 #pragma unroll
@@ -442,37 +451,39 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int columns
 
 struct Plan {
   bool cols;
-  int col_tiles, splits, chunk;
+  int r, col_tiles, splits, chunk;
 };
 
-// Column tiles of a wave that has columns of its own.  (Three terms, or heads of 256: what two take does not fit its registers.)
-static constexpr int wave_tiles(int dtype, int hd) { return dtype == kF32 || hd > 128 ? 1 : 2; }
-
-// Columns a workgroup: 16 shared by its waves, or 64 R of their own.  Keys a workgroup: so that about a thousand workgroups run.
+// How a launch is laid out: a function of its sizes and the rows' type alone.
 static Plan plan(int n_seqs, int nkv, int rep, int hd, int max_q, int max_context, int window, int dtype) {
   Plan p;
   const long long columns = (long long)max_q * rep;
   p.cols = columns > 32;
-  const int width = p.cols ? 64 * wave_tiles(dtype, hd) : 16, tile = p.cols ? width / 4 : 16;
+  // Waves with columns of their own: two tiles of them where there are many and they fit the registers (2,048 rows of 32 heads of 128: 84 us,
+  // one tile 96; 120 rows of 5 requests, 3 heads a kv head: 7.7 and 5.9; 64 rows behind 8,000, 4 a kv head: 37.7 and 36.5).
+  p.r = p.cols && columns >= 1024 && dtype == kBF16 && hd <= 128 ? 2 : 1;
+  const int width = p.cols ? 64 * p.r : 16;
   p.col_tiles = (int)((columns + width - 1) / width);
-  const long long tokens = std::min<long long>(max_q, (tile - 1) / rep + 2);
+  const long long tokens = std::min<long long>(max_q, (16 * p.r - 1) / rep + 2);
   const long long span = window > 0 ? std::min<long long>(max_context, window + tokens + kTile) : max_context;
+  // Runs of a context: about as many workgroups as compute units (half as many again of four waves), none of fewer than 1,024 keys (256).  us:
+  // 4 requests of 16,000 keys and 8 kv heads in 8 runs 23.6, in 4 29.6, in 16 28.7; 256 workgroups in one run 18.2, in two 21.9; 131 rows behind
+  // 3,900, 32 heads, in 8 30, in 4 34.
   const long long groups = (long long)n_seqs * nkv * p.col_tiles;
-  const int grain = p.cols ? kTile : 4 * kTile;
-  long long want = std::max<long long>(1, std::min<long long>(kMostSplits, 1024 / std::max<long long>(1, groups)));
-  long long chunk = (span + want - 1) / want;
-  chunk = std::max<long long>(256, (chunk + grain - 1) / grain * grain);
+  const long long want = ((p.cols ? 512 : 256) + groups / 2) / groups, least = p.cols ? 256 : 1024, grain = p.cols ? kTile : 8 * kTile;
+  const long long runs = std::max<long long>(1, std::min<long long>(want, kMostSplits));
+  const long long chunk = std::max(least, ((span + runs - 1) / runs + grain - 1) / grain * grain);
   p.splits = (int)std::max<long long>(1, (span + chunk - 1) / chunk);
   p.chunk = (int)chunk;
   return p;
 }
 
 template <typename T, int NB> static void launch(const Plan& p, const AttendArgs& a, int n_seqs, hipStream_t stream) {
-  constexpr int W = 4;
-  constexpr int R = wave_tiles(std::is_same_v<T, float> ? kF32 : kBF16, NB * kFp4Block);
+  constexpr int W = NB == 8 ? 4 : 8;   // (the waves' sums of heads of 256 would not fit LDS twice)
   const dim3 grid((unsigned)((long long)n_seqs * a.nkv * p.col_tiles * p.splits));
-  if (p.cols) hipLaunchKernelGGL((fp4_attend_kernel<T, NB, R, W, true>), grid, dim3(W * kWave), 0, stream, a);
-  else hipLaunchKernelGGL((fp4_attend_kernel<T, NB, 1, NB == 8 ? 2 : W, false>), grid, dim3((NB == 8 ? 2 : W) * kWave), 0, stream, a);
+  if (!p.cols) hipLaunchKernelGGL((fp4_attend_kernel<T, NB, 1, W, false>), grid, dim3(W * kWave), 0, stream, a);
+  else if (p.r == 1) hipLaunchKernelGGL((fp4_attend_kernel<T, NB, 1, 4, true>), grid, dim3(4 * kWave), 0, stream, a);
+  else if constexpr (std::is_same_v<T, bf16> && NB <= 4) hipLaunchKernelGGL((fp4_attend_kernel<T, NB, 2, 4, true>), grid, dim3(4 * kWave), 0, stream, a);
   if (p.splits > 1) {
     const int columns = n_seqs * a.nkv * a.max_q * a.rep;
     hipLaunchKernelGGL((fp4_join_kernel<T, NB * kFp4Block>), dim3((columns + 3) / 4), dim3(256), 0, stream, a, columns);

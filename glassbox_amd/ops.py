@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 import struct
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
@@ -2590,21 +2591,25 @@ class Fp4Matrix(NamedTuple):
 
 def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """The operands lie on the current device, whose stream the kernels are launched on."""
+    here = None
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.get_device() != _get_device()):
-            raise KernelError(f"{what}: operands must be on the current GPU")
+        if t is not None:
+            at = t.get_device()   # (-1: not on a GPU)
+            if at < 0 or at != (here := _get_device() if here is None else here):
+                raise KernelError(f"{what}: operands must be on the current GPU")
 
 
-def _span(t: torch.Tensor):
-    at = t.data_ptr()
-    return at, at + (1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else at
+def _end(t: torch.Tensor, at: int) -> int:
+    """Where the memory of a tensor that begins at ``at`` ends."""
+    return at + (1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else at
 
 
 def _apart(a: torch.Tensor, b: torch.Tensor, what: str, same: bool = False) -> None:
     """The two share no memory; with ``same`` they may be rows at the same places."""
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    if a0 < b1 and b0 < a1 and not (same and a0 == b0 and a.stride() == b.stride()):
-        raise KernelError(what)
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    if _end(a, a0) > b0 if a0 < b0 else _end(b, b0) > a0:
+        if not (same and a0 == b0 and a.stride() == b.stride()):
+            raise KernelError(what)
 
 
 def fp4_scale_bytes(columns: int) -> int:
@@ -2620,14 +2625,16 @@ def fp4_pages_shape(pages: int, n_kv_heads: int, page_size: int, head_dim: int) 
 
 
 def _fp4_pages(k_pages, v_pages, what: str):
-    """(pages, kv heads, page size, head size) of four-bit pages."""
-    if (k_pages is None or v_pages is None or k_pages.dim() != 5 or k_pages.shape != v_pages.shape or k_pages.shape[3] != 17
-            or k_pages.shape[4] % 16 or 0 in k_pages.shape or k_pages.dtype != torch.uint8 or v_pages.dtype != torch.uint8
-            or not k_pages.is_contiguous() or not v_pages.is_contiguous() or k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16):
-        raise KernelError(f"{what}: four-bit pages are contiguous uint8 [pages, kv heads, head size / 32, 17, page size], of a multiple of "
-                          f"16 slots, keys and values alike")
-    p, h, nb, _, s = k_pages.shape
-    return p, h, s, nb * FP4_BLOCK
+    """(pages, kv heads, page size, head size, where the keys' and the values' begin) of four-bit pages."""
+    if k_pages is not None and v_pages is not None:
+        shape, k_at, v_at = k_pages.shape, k_pages.data_ptr(), v_pages.data_ptr()
+        if (len(shape) == 5 and v_pages.shape == shape and shape[3] == 17 and shape[4] % 16 == 0 and k_pages.dtype == torch.uint8
+                and v_pages.dtype == torch.uint8 and k_pages.is_contiguous() and v_pages.is_contiguous() and (k_at | v_at) % 16 == 0):
+            p, h, nb, _, s = shape
+            if p and h and nb and s:
+                return p, h, s, nb * FP4_BLOCK, k_at, v_at
+    raise KernelError(f"{what}: four-bit pages are contiguous uint8 [pages, kv heads, head size / 32, 17, page size], of a multiple of "
+                      f"16 slots, keys and values alike")
 
 
 def fp4_store(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], slots: Optional[torch.Tensor],
@@ -2638,24 +2645,28 @@ def fp4_store(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torc
     turned in 32 bits, and its value heads go to the pages at ``slots`` as the nearest four-bit numbers.  The keys and values of ``qkv``
     are left as they are.  ``slots`` None: nothing is stored.  A row whose slot is negative or beyond the pages is not stored; the slots of
     the others must differ."""
-    n = qkv.shape[0]
     stride = _rows(qkv, "qkv")
-    width = (n_heads + 2 * n_kv_heads) * head_dim
+    n, given = qkv.shape
     if n_heads < 0 or n_kv_heads < 0 or head_dim <= 0 or head_dim % FP4_BLOCK:
         raise KernelError(f"fp4_store: {n_heads} and {n_kv_heads} heads of {head_dim} channels: a multiple of {FP4_BLOCK} is needed")
-    if qkv.shape[1] < width:
-        raise KernelError(f"fp4_store: rows of {qkv.shape[1]} do not hold {n_heads} + 2 * {n_kv_heads} heads of {head_dim}")
+    if given < (n_heads + 2 * n_kv_heads) * head_dim:
+        raise KernelError(f"fp4_store: rows of {given} do not hold {n_heads} + 2 * {n_kv_heads} heads of {head_dim}")
     pages = page_size = 0
+    k_at = v_at = slots_at = cos_at = sin_at = None
     if slots is not None:
         _i32(slots, "slots", n)
-        pages, p_heads, page_size, p_hd = _fp4_pages(k_pages, v_pages, "fp4_store")
-        if (p_heads, p_hd) != (n_kv_heads, head_dim):
+        pages, p_heads, page_size, p_hd, k_at, v_at = _fp4_pages(k_pages, v_pages, "fp4_store")
+        if p_heads != n_kv_heads or p_hd != head_dim:
             raise KernelError("fp4_store: pages do not have this layer's kv heads and head size")
-    if (cos is None) != (sin is None):
+        slots_at = slots.data_ptr()
+    if cos is not None and sin is not None:
+        for t in (cos, sin):
+            shape = t.shape
+            if t.dtype != torch.float32 or not t.is_contiguous() or len(shape) != 2 or shape[0] < n or shape[1] != head_dim // 2:
+                raise KernelError("fp4_store: cos/sin must be contiguous float32 [n, head_dim/2]")
+        cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+    elif cos is not None or sin is not None:
         raise KernelError("fp4_store: cosines and sines go together")
-    for t in (cos, sin):
-        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or t.shape[0] < n or t.shape[1] != head_dim // 2):
-            raise KernelError("fp4_store: cos/sin must be contiguous float32 [n, head_dim/2]")
     if q is None:
         q, q_stride = qkv, stride
     else:
@@ -2666,14 +2677,14 @@ def fp4_store(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torc
     dtype = dtype_code(qkv)
     _here("fp4_store", qkv, cos, sin, slots, k_pages, v_pages, q)
     lib = _lib("fp4_cache")
-    _launch(lib, lib.gb_fp4_store, _p(qkv), dtype, stride, _p(q), q_stride, _p(cos), _p(sin), _p(slots), _p(k_pages), _p(v_pages),
-            n, n_heads, n_kv_heads, head_dim, page_size, pages, _stream())
+    _launch(lib, lib.gb_fp4_store, qkv.data_ptr(), dtype, stride, q.data_ptr(), q_stride, cos_at, sin_at, slots_at, k_at, v_at, n, n_heads,
+            n_kv_heads, head_dim, page_size, pages, _stream())
 
 
 def fp4_load(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
     """The keys and values that four-bit pages hold at ``slots``, as the values they stand for: ``k``, ``v`` [n, kv heads * head size],
     bfloat16 (exact) or float32.  Rows whose slot is negative or beyond the pages are left as they are."""
-    pages, nkv, page_size, hd = _fp4_pages(k_pages, v_pages, "fp4_load")
+    pages, nkv, page_size, hd, k_at, v_at = _fp4_pages(k_pages, v_pages, "fp4_load")
     n = k.shape[0]
     _i32(slots, "slots", n)
     if k.dtype != v.dtype or k.shape != (n, nkv * hd) or v.shape != (n, nkv * hd):
@@ -2682,7 +2693,7 @@ def fp4_load(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     dtype, k_stride, v_stride = dtype_code(k), _rows(k, "k"), _rows(v, "v")
     _here("fp4_load", slots, k_pages, v_pages, k, v)
     lib = _lib("fp4_cache")
-    _launch(lib, lib.gb_fp4_load, _p(slots), _p(k_pages), _p(v_pages), _p(k), k_stride, _p(v), v_stride, dtype, n, nkv, hd, page_size,
+    _launch(lib, lib.gb_fp4_load, slots.data_ptr(), k_at, v_at, k.data_ptr(), k_stride, v.data_ptr(), v_stride, dtype, n, nkv, hd, page_size,
             pages, _stream())
 
 
@@ -2706,30 +2717,41 @@ def fp4_attention(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_l
     position is negative, its pages' numbers are none of the pool's) gives zeros; what lies in a masked place, not finite or not, does not
     matter.  bfloat16 or float32 rows; heads of 32, 64, 96, 128 or 256 channels; a positive scale.
     ``workspace`` (float32, ``fp4_attention_floats`` elements): needed where that is not 0."""
-    pages, nkv, page_size, hd = _fp4_pages(k_pages, v_pages, "fp4_attention")
-    n = q.shape[0]
-    if q.dtype != out.dtype or q.dim() != 2 or q.shape[1] != n_heads * hd or out.shape != q.shape:
+    pages, nkv, page_size, hd, k_at, v_at = _fp4_pages(k_pages, v_pages, "fp4_attention")
+    q_stride, out_stride, shape = _rows(q, "q"), _rows(out, "out"), q.shape
+    if q.dtype != out.dtype or shape[1] != n_heads * hd or out.shape != shape:
         raise KernelError(f"fp4_attention: q and out must be [n, {n_heads} heads * {hd}] of one type")
     if hd not in FP4_HEAD_DIMS or n_heads <= 0 or n_heads % nkv:
         raise KernelError(f"fp4_attention: {n_heads} query heads of {hd} channels over {nkv} kv heads: heads of {FP4_HEAD_DIMS}, a multiple of the kv heads")
-    if not 0 < scale < float("inf"):
+    if not 0 < scale < math.inf:
         raise KernelError(f"fp4_attention: a positive scale is needed, got {scale}")
     seqs = q_len.numel()
-    for name, t in (("q_start", q_start), ("q_len", q_len), ("pos0", pos0)):
-        _i32(t, name, seqs)
-    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.stride(1) != 1 or tables.shape[0] < seqs or tables.shape[1] == 0:
+    _i32(q_start, "q_start", seqs)
+    _i32(q_len, "q_len", seqs)
+    _i32(pos0, "pos0", seqs)
+    tables_shape = tables.shape
+    if tables.dtype != torch.int32 or len(tables_shape) != 2 or tables.stride(1) != 1 or tables_shape[0] < seqs or tables_shape[1] == 0:
         raise KernelError("fp4_attention: block tables must be int32 [requests, pages]")
-    if window < 0 or max_q_len < 0 or max_context < 0:
-        raise KernelError("fp4_attention: a window, a number of rows or a context below 0")
+    window, max_q_len, max_context = int(window), int(max_q_len), int(max_context)
+    if not (0 <= window < 1 << 31 and 0 <= max_q_len < 1 << 31 and 0 <= max_context < 1 << 31):
+        raise KernelError("fp4_attention: a window, a number of rows or a context below 0 or beyond 32 bits")
     _apart(q, out, "fp4_attention: out lies over other rows of q", same=True)
-    if workspace is not None and (workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.data_ptr() % 16):
-        raise KernelError("fp4_attention: the workspace must be contiguous float32 that begins at a 16-byte word")
-    dtype, q_stride, out_stride = dtype_code(q), _rows(q, "q"), _rows(out, "out")
+    ws_at, ws_floats = _fp4_workspace(workspace, "fp4_attention")
+    dtype = dtype_code(q)
     _here("fp4_attention", q, out, q_start, q_len, pos0, tables, k_pages, v_pages, workspace)
     lib = _lib("fp4_attention")
-    _launch(lib, lib.gb_fp4_attention, _p(q), q_stride, _p(out), out_stride, dtype, n, _p(q_start), _p(q_len), _p(pos0), seqs,
-            int(max_q_len), int(max_context), _p(tables), tables.stride(0), tables.shape[1], _p(k_pages), _p(v_pages), pages, n_heads, nkv, hd,
-            page_size, float(scale), int(window), _p(workspace), workspace.numel() if workspace is not None else 0, _stream())
+    _launch(lib, lib.gb_fp4_attention, q.data_ptr(), q_stride, out.data_ptr(), out_stride, dtype, shape[0], q_start.data_ptr(), q_len.data_ptr(),
+            pos0.data_ptr(), seqs, max_q_len, max_context, tables.data_ptr(), tables.stride(0), tables_shape[1], k_at, v_at, pages, n_heads, nkv, hd,
+            page_size, scale, window, ws_at, ws_floats, _stream())
+
+
+def _fp4_workspace(workspace: Optional[torch.Tensor], what: str) -> Tuple[Optional[int], int]:
+    if workspace is None:
+        return None, 0
+    at = workspace.data_ptr()
+    if workspace.dtype != torch.float32 or not workspace.is_contiguous() or at % 16:
+        raise KernelError(f"{what}: the workspace must be contiguous float32 that begins at a 16-byte word")
+    return at, workspace.numel()
 
 
 def fp4_quantize(w: torch.Tensor) -> Fp4Matrix:
@@ -2747,25 +2769,27 @@ def fp4_quantize(w: torch.Tensor) -> Fp4Matrix:
     return m
 
 
-def _fp4_matrix(w: Fp4Matrix, what: str) -> Tuple[int, int]:
+def _fp4_matrix(w: Fp4Matrix, what: str) -> Tuple[int, int, int, int, int]:
+    """(rows, columns, scales a row, where codes and scales begin) of a four-bit matrix."""
     codes, scales = w
-    if (codes.dim() != 2 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_contiguous() or not scales.is_contiguous()
-            or codes.shape[1] % 16 or 0 in codes.shape or scales.shape != (codes.shape[0], fp4_scale_bytes(2 * codes.shape[1]))
-            or codes.data_ptr() % 16 or scales.data_ptr() % 16):
-        raise KernelError(f"{what}: a four-bit matrix has contiguous uint8 codes [rows, columns / 2] and scales [rows, columns / 32 filled up to a "
-                          f"multiple of 16], got {tuple(codes.shape)} and {tuple(scales.shape)}")
-    return w.shape
+    if codes.dim() == 2 and scales.dim() == 2:
+        (n, half), (m, each), c_at, s_at = codes.shape, scales.shape, codes.data_ptr(), scales.data_ptr()
+        if (n > 0 and half > 0 and half % 16 == 0 and m == n and each == (half // 16 + 15) // 16 * 16 and codes.dtype == torch.uint8
+                and scales.dtype == torch.uint8 and codes.is_contiguous() and scales.is_contiguous() and (c_at | s_at) % 16 == 0):
+            return n, 2 * half, each, c_at, s_at
+    raise KernelError(f"{what}: a four-bit matrix has contiguous uint8 codes [rows, columns / 2] and scales [rows, columns / 32 filled up to a "
+                      f"multiple of 16], got {tuple(codes.shape)} and {tuple(scales.shape)}")
 
 
 def fp4_expand(w: Fp4Matrix, out: torch.Tensor) -> None:
     """The values of a four-bit matrix: ``out`` [rows, columns], contiguous, bfloat16 (exact) or float32."""
-    n, k = _fp4_matrix(w, "fp4_expand")
+    n, k, each, c_at, s_at = _fp4_matrix(w, "fp4_expand")
     if out.shape != (n, k) or not out.is_contiguous() or out.data_ptr() % 16:
         raise KernelError(f"fp4_expand: out must be contiguous [{n}, {k}] and begin at a 16-byte word")
     dtype = dtype_code(out)
     _here("fp4_expand", *w, out)
     lib = _lib("fp4_cache")
-    _launch(lib, lib.gb_fp4_expand, _p(w.codes), _p(w.scales), _p(out), dtype, n, k, w.scales.shape[1], _stream())
+    _launch(lib, lib.gb_fp4_expand, c_at, s_at, out.data_ptr(), dtype, n, k, each, _stream())
 
 
 def _fp4_expands(rows: int, n: int, k: int, dtype: torch.dtype, out_dtype: torch.dtype, silu_mul: bool) -> bool:
@@ -2793,25 +2817,23 @@ def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool 
     many columns.
     ``workspace`` (float32, ``fp4_gemm_floats`` elements; optional): lets few workgroups divide k (their sums are added in a fixed order), and
     large bfloat16 products have the weights' bfloat16 values written there first and multiplied by ``gemm``."""
-    N, K = _fp4_matrix(w, "fp4_gemm")
-    if a.dim() != 2 or a.shape[1] != K or out.shape != (a.shape[0], N // 2 if silu_mul else N):
+    N, K, each, c_at, s_at = _fp4_matrix(w, "fp4_gemm")
+    lda, ldo, (M, k) = _rows(a, "a"), _rows(out, "out"), a.shape
+    if k != K or out.shape != (M, N // 2 if silu_mul else N):
         raise KernelError(f"fp4_gemm: shapes do not match: a {tuple(a.shape)}, w {(N, K)}, out {tuple(out.shape)}")
     if silu_mul and (accumulate or N % 2):
         raise KernelError("fp4_gemm: the fused SiLU-multiply takes an even number of rows of w and does not accumulate")
     if accumulate and out.dtype != torch.float32:
         raise KernelError("fp4_gemm: accumulation is into a 32-bit result")
     _apart(a, out, "fp4_gemm: a and out share memory")
-    if workspace is not None and (workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.data_ptr() % 16):
-        raise KernelError("fp4_gemm: the workspace must be contiguous float32 that begins at a 16-byte word")
-    lda, ldo, dtype, out_dtype = _rows(a, "a"), _rows(out, "out"), dtype_code(a), dtype_code(out)
-    _here("fp4_gemm", a, *w, out, workspace)
-    M, floats = a.shape[0], workspace.numel() if workspace is not None else 0
+    ws_at, floats = _fp4_workspace(workspace, "fp4_gemm")
+    dtype, out_dtype = dtype_code(a), dtype_code(out)
+    _here("fp4_gemm", a, w.codes, w.scales, out, workspace)
     if floats >= N * K // 2 and _fp4_expands(M, N, K, a.dtype, out.dtype, silu_mul) and lda % 8 == 0 and a.data_ptr() % 16 == 0:
-        values = workspace[:N * K // 2].view(torch.bfloat16).view(N, K)
-        rest = workspace[N * K // 2:]
+        values, rest = workspace[:N * K // 2].view(torch.bfloat16).view(N, K), workspace[N * K // 2:]
         fp4_expand(w, values)
         gemm(a, values, out, accumulate=accumulate, silu_mul=silu_mul, workspace=rest if rest.numel() >= max(1, gemm_split_floats(M, N, K)) else None)
         return
     lib = _lib("fp4_gemm")
-    _launch(lib, lib.gb_fp4_gemm, _p(a), dtype, lda, _p(w.codes), _p(w.scales), w.scales.shape[1], _p(out), out_dtype, ldo, M, N, K,
-            2 if silu_mul else 1 if accumulate else 0, _p(workspace), floats, _stream())
+    _launch(lib, lib.gb_fp4_gemm, a.data_ptr(), dtype, lda, c_at, s_at, each, out.data_ptr(), out_dtype, ldo, M, N, K,
+            2 if silu_mul else 1 if accumulate else 0, ws_at, floats, _stream())
