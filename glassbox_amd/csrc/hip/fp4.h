@@ -98,24 +98,31 @@ __device__ __forceinline__ void store8(float* p, bool wide, const float (&x)[8])
   }
 }
 
-// A 32-bit operand of a product on the bf16 matrix cores: the sum of three bf16 numbers, each the nearest to what the ones
-// before leave (3 x 8 bits of mantissa hold all 24).  The other operand is exact in bf16, so that the three products are
-// exact and their sum is rounded in 32 bits alone.  A number that is not finite goes into the first term, the others being zero.
+// A 32-bit operand of a product on the bf16 matrix cores: the sum of three bf16 numbers, the bits of the mantissa in three runs of
+// eight.  The other operand is exact in bf16, so that the three products are exact and their sum is rounded in 32 bits alone.  A number
+// that is not finite goes into the first term, the others being zero.
 template <typename T> constexpr int kFp4Terms = std::is_same_v<T, float> ? 3 : 1;
-template <int N> __device__ __forceinline__ void fp4_terms(const float (&x)[8], bf16x8 (&out)[N]) {
+__device__ __forceinline__ void fp4_terms(const float (&x)[8], bf16x8 (&out)[3]) {
+  uint32_t t[3][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float rest = x[i];
-#pragma unroll
-    for (int t = 0; t < N; ++t) {
-      const bf16 h = (bf16)rest;
-      out[t][i] = h;
-      if (t + 1 < N) {
-        const float left = rest - (float)h;
-        rest = fabsf(left) < __builtin_inff() ? left : 0.f;   // (infinity less itself; a number that rounded up to infinity)
-      }
-    }
+    const float v = __builtin_canonicalizef(x[i]);   // (the mark of a NaN may lie in the low bits)
+    t[0][i] = __float_as_uint(v);
+    const float left = v - __uint_as_float(t[0][i] & 0xffff0000u), rest = fabsf(v) < __builtin_inff() ? left : 0.f;
+    t[1][i] = __float_as_uint(rest);
+    t[2][i] = __float_as_uint(rest - __uint_as_float(t[1][i] & 0xffff0000u));
   }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(t[k][2 * i + 1], t[k][2 * i], 0x07060302u);   // the upper halves
+    __builtin_memcpy(&out[k], w, sizeof w);
+  }
+}
+__device__ __forceinline__ void fp4_terms(const float (&x)[8], bf16x8 (&out)[1]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) out[0][i] = (bf16)x[i];
 }
 
 }  // namespace gb

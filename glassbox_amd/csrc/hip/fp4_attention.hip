@@ -145,7 +145,7 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(COLS 
         float x[8];
         load8(row + (g + 4 * i) * U::kChannels + 8 * w, a.q_wide, x);
         bf16x8 terms[SP];
-        fp4_terms<SP>(x, terms);
+        fp4_terms(x, terms);
 #pragma unroll
         for (int p = 0; p < SP; ++p) qf[t][p][i * U::kWords + w] = terms[p];
       }
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(COLS 
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = p[8 * c + e];
         bf16x8 terms[SP];
-        fp4_terms<SP>(x, terms);
+        fp4_terms(x, terms);
 #pragma unroll
         for (int q = 0; q < SP; ++q) pf[t][q][c] = terms[q];
       }

@@ -20,6 +20,21 @@ __device__ __forceinline__ uint32_t largest8(const float (&x)[8]) {
   return m;
 }
 
+// Four neighbouring lanes hold four bytes each: lane i gets the four bytes i, in the order of the lanes.
+__device__ __forceinline__ uint32_t turn_bytes(uint32_t w, int lane) {
+  const uint32_t a = (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0xb1, 0xf, 0xf, true);   // of lane ^ 1
+  w = lane & 1 ? __builtin_amdgcn_perm(w, a, 0x07030501u) : __builtin_amdgcn_perm(a, w, 0x06020400u);
+  const uint32_t b = (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0x4e, 0xf, 0xf, true);   // of lane ^ 2
+  return lane & 2 ? __builtin_amdgcn_perm(w, b, 0x07060302u) : __builtin_amdgcn_perm(b, w, 0x05040100u);
+}
+// Whether the slots of this lane and its three neighbours (tokens 4 i .. 4 i + 3) are four in a row from a multiple of four on: their
+// bytes in a row of values are then one word.  All lanes take part.
+__device__ __forceinline__ bool quad_in_a_row(int slot, bool stored, int lane) {
+  const int first = __builtin_amdgcn_mov_dpp(slot, 0x00, 0xf, 0xf, true);
+  const bool fits = stored && slot - (lane & 3) == first && (first & 3) == 0;
+  return (__ballot(fits) >> (lane & ~3) & 15) == 15;
+}
+
 struct StoreArgs {
   const void* qkv;
   void* q;
@@ -27,93 +42,141 @@ struct StoreArgs {
   const int32_t* slots;
   uint8_t *k, *v;
   int stride, q_stride, n, nh, nkv, hd, page, pages, wide, q_wide, cs_wide;
-  int kv_blocks;   // workgroups that store; the others turn queries
+  int kv_blocks, k_units, v_units;   // workgroups that store, the others turn queries; units of 16 tokens' keys and of their values
 };
 
-// Keys and values: a wave takes one block of 32 channels of 16 tokens, lane l tokens l % 16 and the channels' quarter l / 16, so that
-// what 16 neighbouring tokens bring lies side by side in both kinds of pages: a store of keys fills 256 bytes, one of values four
-// runs of 16.  (A lane a whole block would have the rows' reads in whole lines, and the values' bytes in stores of one token each.)
+// Keys and values: a wave takes 16 tokens, lane l token l % 16 and of a block of 32 channels the quarter l / 16, so that what neighbouring
+// tokens bring lies side by side in both kinds of pages: a store of keys fills 256 bytes, and so does one of values where the tokens' slots
+// follow each other (their bytes are exchanged between four lanes).  Keys of heads of 64 channels and multiples go two blocks at a time,
+// (i, i + hd / 2).  A lane takes kHeads heads, which share their angles, one after the other: 6,151 rows of 8 kv heads of 128 in 11 us, a head at a
+// time and values byte by byte in 21; with the queries of 32 heads 27 and 39.  The few rows of a decode step take one: 3.6 us, four 4.6.
 // Queries: a lane takes 8 pairs (i, i + hd / 2) and may write where it read.
-template <typename T>
+template <typename T, bool PAIRS, int kHeads>
 __global__ __launch_bounds__(256) void fp4_store_kernel(StoreArgs a) {
   const int lane = threadIdx.x % kWave, half = a.hd / 2;
   if ((int)blockIdx.x < a.kv_blocks) {
-    const int nb = a.hd / kFp4Block, units = 2 * a.nkv * nb;
+    const int nb = a.hd / kFp4Block, units = a.k_units + a.v_units;
     const int wave = blockIdx.x * 4 + threadIdx.x / kWave;
-    const int unit = wave % units, group = wave / units;
-    const int t = group * 16 + lane % 16, quarter = lane / 16;
+    int unit = wave % units;
+    const int group = wave / units, t = group * 16 + lane % 16, quarter = lane / 16;
     if (group * 16 >= a.n) return;
-    const int slot = t < a.n ? a.slots[t] : -1;
+    const int row = min(t, a.n - 1), slot = t < a.n ? a.slots[t] : -1;
     const bool stored = slot >= 0 && slot / a.page < a.pages;
-    const int row = t < a.n ? t : a.n - 1;
-    const int head = unit / nb, b = unit % nb;   // keys' heads, then values'
-    const T* src = (const T*)a.qkv + (size_t)row * a.stride + (size_t)(a.nh + head) * a.hd;
-    const int c = b * kFp4Block + quarter * 8;
-    float x[8];
-    load8(src + c, a.wide, x);
-    if (head < a.nkv && a.cosv) {
-      const bool low = c < half;
-      float other[8], cs[8], sn[8];
-      load8(src + (low ? c + half : c - half), a.wide, other);
-      const size_t at = (size_t)row * half + (low ? c : c - half);
-      load8(a.cosv + at, a.cs_wide, cs);
-      load8(a.sinv + at, a.cs_wide, sn);
+    const int page = stored ? slot / a.page : 0, off = stored ? slot % a.page : 0;
+    const size_t block = fp4_block_bytes(a.page), head_bytes = block * nb;
+    if (unit < a.k_units) {
+      constexpr int B = PAIRS ? 2 : 1;
+      const int per = PAIRS ? nb / 2 : nb, head0 = unit / per * kHeads, b = unit % per;
+      const int c = b * kFp4Block + quarter * 8;                       // and with PAIRS c + half
+      const bool low = PAIRS || c < half;
+      const int other = low ? c + half : c - half, angle = low ? c : other;
+      const T* src = (const T*)a.qkv + (size_t)row * a.stride + (size_t)a.nh * a.hd;
+      uint8_t* dst = a.k + (size_t)page * a.nkv * head_bytes + (size_t)b * block;
+      float cs[8], sn[8], x[kHeads][8], y[kHeads][8];
+      if (a.cosv) {
+        load8(a.cosv + (size_t)row * half + angle, a.cs_wide, cs);
+        load8(a.sinv + (size_t)row * half + angle, a.cs_wide, sn);
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = low ? turned_lo(x[i], other[i], cs[i], sn[i]) : turned_hi(other[i], x[i], cs[i], sn[i]);
+      for (int h = 0; h < kHeads; ++h) {
+        const T* p = src + (size_t)min(head0 + h, a.nkv - 1) * a.hd;
+        load8(p + c, a.wide, x[h]);
+        if (PAIRS || a.cosv) load8(p + other, a.wide, y[h]);
+      }
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+        if (head0 + h >= a.nkv) return;
+        if (a.cosv) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float lo = low ? x[h][i] : y[h][i], hi = low ? y[h][i] : x[h][i];
+            const float first = turned_lo(lo, hi, cs[i], sn[i]), second = turned_hi(lo, hi, cs[i], sn[i]);
+            x[h][i] = low ? first : second;
+            y[h][i] = second;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+          const float(&z)[8] = k ? y[h] : x[h];
+          const uint32_t byte = fp4_scale_byte(quarters_max(largest8(z))), word = fp4_pack8(z, fp4_unit(byte));
+          uint8_t* to = dst + (size_t)(head0 + h) * head_bytes + (size_t)(k * (nb / 2)) * block;
+          if (stored) {
+            *reinterpret_cast<uint32_t*>(to + off * 16 + quarter * 4) = word;
+            if (quarter == 0) to[16 * a.page + fp4_key_scale_place(off)] = (uint8_t)byte;
+          }
+        }
+      }
+      return;
     }
-    const uint32_t byte = fp4_scale_byte(quarters_max(largest8(x)));
-    uint32_t word = fp4_pack8(x, fp4_unit(byte));
-    const int page = slot / a.page, off = slot % a.page;
-    const size_t block = fp4_block_bytes(a.page);
-    if (head < a.nkv) {
-      if (!stored) return;
-      uint8_t* dst = a.k + (((size_t)page * a.nkv + head) * nb + b) * block;
-      *reinterpret_cast<uint32_t*>(dst + off * 16 + quarter * 4) = word;
-      if (quarter == 0) dst[16 * a.page + fp4_key_scale_place(off)] = (uint8_t)byte;
-    } else {
-      // bytes of channels (i, i + 16): quarters 0 and 2 have the halves of rows 0..7, quarters 1 and 3 of rows 8..15; after the
-      // exchange every lane has four rows to write
-      const uint32_t theirs = __shfl_xor(word, 32, kWave);
-      const uint32_t lo = quarter < 2 ? word : theirs, hi = quarter < 2 ? theirs : word;
-      const int first = (quarter & 1) * 8 + (quarter >> 1) * 4, shift = (quarter >> 1) * 16;
-      if (!stored) return;
-      uint8_t* dst = a.v + (((size_t)page * a.nkv + head - a.nkv) * nb + b) * block + off;
+    unit -= a.k_units;
+    const int head0 = unit / nb * kHeads, b = unit % nb;
+    const T* src = (const T*)a.qkv + (size_t)row * a.stride + (size_t)(a.nh + a.nkv) * a.hd + b * kFp4Block + quarter * 8;
+    uint8_t* dst = a.v + (size_t)page * a.nkv * head_bytes + (size_t)b * block;
+    const bool words = quad_in_a_row(slot, stored, lane);
+    float x[kHeads][8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        dst[(size_t)(first + i) * a.page] = (uint8_t)(((lo >> (shift + 4 * i)) & 15u) | (((hi >> (shift + 4 * i)) & 15u) << 4));
-      if (quarter == 0) dst[(size_t)16 * a.page] = (uint8_t)byte;
+    for (int h = 0; h < kHeads; ++h) load8(src + (size_t)min(head0 + h, a.nkv - 1) * a.hd, a.wide, x[h]);
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      if (head0 + h >= a.nkv) return;
+      const uint32_t byte = fp4_scale_byte(quarters_max(largest8(x[h]))), word = fp4_pack8(x[h], fp4_unit(byte));
+      // bytes of channels (i, i + 16): quarters 0 and 2 have the halves of rows 0..7, quarters 1 and 3 of rows 8..15; after the exchange every
+      // lane has four rows of its token
+      const uint32_t theirs = __shfl_xor(word, 32, kWave);
+      const int shift = (quarter >> 1) * 16, first = (quarter & 1) * 8 + (quarter >> 1) * 4;
+      const uint32_t lo = (quarter < 2 ? word : theirs) >> shift, hi = (quarter < 2 ? theirs : word) >> shift;
+      uint32_t four = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) four |= ((lo >> (4 * i) & 15u) | (hi >> (4 * i) & 15u) << 4) << (8 * i);
+      const uint32_t turned = turn_bytes(four, lane);
+      uint8_t* to = dst + (size_t)(head0 + h) * head_bytes;
+      if (words) {
+        *reinterpret_cast<uint32_t*>(to + (size_t)(first + (lane & 3)) * a.page + (off & ~3)) = turned;
+      } else if (stored) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[(size_t)(first + i) * a.page + off] = (uint8_t)(four >> (8 * i));
+      }
+      if (stored && quarter == 0) to[(size_t)16 * a.page + off] = (uint8_t)byte;
     }
     return;
   }
-  const int pieces = half / 8;
+  // queries
+  const int pieces = half / 8, groups = (a.nh + kHeads - 1) / kHeads;
   const long long item = (long long)(blockIdx.x - a.kv_blocks) * 256 + threadIdx.x;
-  const int t = (int)(item / (a.nh * pieces)), rest = (int)(item % (a.nh * pieces));
+  const int t = (int)(item / (groups * pieces)), rest = (int)(item % (groups * pieces));
   if (t >= a.n) return;
-  const int head = rest / pieces, c = rest % pieces * 8;
-  const T* src = (const T*)a.qkv + (size_t)t * a.stride + (size_t)head * a.hd + c;
-  T* dst = (T*)a.q + (size_t)t * a.q_stride + (size_t)head * a.hd + c;
-  float x0[8], x1[8];
-  load8(src, a.wide, x0);
-  load8(src + half, a.wide, x1);
+  const int head0 = rest / pieces * kHeads, c = rest % pieces * 8;
+  const T* src = (const T*)a.qkv + (size_t)t * a.stride + c;
+  T* dst = (T*)a.q + (size_t)t * a.q_stride + c;
+  float cs[8], sn[8], x0[kHeads][8], x1[kHeads][8];
   if (a.cosv) {
-    float cs[8], sn[8], y0[8], y1[8];
     load8(a.cosv + (size_t)t * half + c, a.cs_wide, cs);
     load8(a.sinv + (size_t)t * half + c, a.cs_wide, sn);
+  }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      y0[i] = turned_lo(x0[i], x1[i], cs[i], sn[i]);
-      y1[i] = turned_hi(x0[i], x1[i], cs[i], sn[i]);
+  for (int h = 0; h < kHeads; ++h) {   // (a last group that is not full reads its last head again)
+    const T* p = src + (size_t)min(head0 + h, a.nh - 1) * a.hd;
+    load8(p, a.wide, x0[h]);
+    load8(p + half, a.wide, x1[h]);
+  }
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (head0 + h >= a.nh) return;
+    if (a.cosv) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float lo = turned_lo(x0[h][i], x1[h][i], cs[i], sn[i]);
+        x1[h][i] = turned_hi(x0[h][i], x1[h][i], cs[i], sn[i]);
+        x0[h][i] = lo;
+      }
     }
-    store8(dst, a.q_wide, y0);
-    store8(dst + half, a.q_wide, y1);
-  } else {
-    store8(dst, a.q_wide, x0);
-    store8(dst + half, a.q_wide, x1);
+    store8(dst + (size_t)(head0 + h) * a.hd, a.q_wide, x0[h]);
+    store8(dst + (size_t)(head0 + h) * a.hd + half, a.q_wide, x1[h]);
   }
 }
 
-// Rows back from their slots: the lanes of a wave as above.  A lane takes eight channels, a word of a key, or a byte of eight rows of
-// values of which it needs one half.
+// Rows back from their slots: the lanes of a wave as above.  A lane takes eight channels: a word of a key; of values a byte of eight rows, of
+// which it needs one half.
 template <typename T>
 __global__ __launch_bounds__(256) void fp4_load_kernel(const int32_t* __restrict__ slots, const uint8_t* __restrict__ k_pages,
                                                       const uint8_t* __restrict__ v_pages, T* __restrict__ k, T* __restrict__ v,
@@ -122,8 +185,7 @@ __global__ __launch_bounds__(256) void fp4_load_kernel(const int32_t* __restrict
   const int nb = hd / kFp4Block, units = 2 * nkv * nb, lane = threadIdx.x % kWave;
   const int wave = blockIdx.x * 4 + threadIdx.x / kWave;
   const int unit = wave % units, t = wave / units * 16 + lane % 16, quarter = lane / 16;
-  if (t >= n) return;
-  const int slot = slots[t];
+  const int slot = t < n ? slots[t] : -1;
   if (slot < 0 || slot / page >= pages) return;
   const int head = unit / nb % nkv, b = unit % nb, off = slot % page;
   const uint8_t* block = (unit < nkv * nb ? k_pages : v_pages) + (((size_t)(slot / page) * nkv + head) * nb + b) * fp4_block_bytes(page);
@@ -133,6 +195,7 @@ __global__ __launch_bounds__(256) void fp4_load_kernel(const int32_t* __restrict
     word = *reinterpret_cast<const uint32_t*>(block + off * 16 + quarter * 4);
     unit_of = fp4_unit(block[16 * page + fp4_key_scale_place(off)]);
   } else {
+    // (byte by byte: words exchanged between four lanes, as the store does it, take 15 us for 6,151 rows of 8 heads of 128, this 12)
 #pragma unroll
     for (int i = 0; i < 8; ++i) word |= ((uint32_t)block[((quarter & 1) * 8 + i) * page + off] >> (quarter >= 2 ? 4 : 0) & 15u) << (4 * i);
     unit_of = fp4_unit(block[16 * page + off]);
@@ -200,15 +263,25 @@ extern "C" int gb_fp4_store(const void* qkv, int dtype, int stride, void* q, int
   GB_REQUIRE(dtype == kF32 || dtype == kBF16, "fp4_store: unknown dtype %d", dtype);
   const int e = dtype == kF32 ? 4 : 2;
   const bool turns = q && nh > 0 && (cosv || q != qkv);
-  const long long waves = slots ? (long long)((n + 15) / 16) * 2 * nkv * (hd / 32) : 0;
-  const long long kv = (waves + 3) / 4, items = turns ? (long long)n * nh * (hd / 16) : 0, blocks = kv + (items + 255) / 256;
+  // four heads a lane where that leaves four waves to a compute unit
+  const bool pairs = hd % 64 == 0;
+  const int each = (long long)((n + 15) / 16) * (nkv + (nh + 3) / 4) * (hd / 32) >= 1024 ? 4 : 1;
+  const int head_groups = (nkv + each - 1) / each, k_units = head_groups * (pairs ? hd / 64 : hd / 32), v_units = head_groups * (hd / 32);
+  const long long waves = slots ? (long long)((n + 15) / 16) * (k_units + v_units) : 0;
+  const long long kv = (waves + 3) / 4, items = turns ? (long long)n * ((nh + each - 1) / each) * (hd / 16) : 0, blocks = kv + (items + 255) / 256;
   if (n == 0 || blocks == 0) return 0;
   GB_REQUIRE(blocks < (1ll << 31) && waves < (1ll << 31), "fp4_store: %d rows are too many for one launch", n);
-  StoreArgs a{qkv, q, cosv, sinv, slots, (uint8_t*)k_pages, (uint8_t*)v_pages, stride, q_stride, n, nh, nkv, hd, page, pages,
-              aligned16(qkv) && (size_t)stride * e % 16 == 0, aligned16(q) && (size_t)q_stride * e % 16 == 0,
-              aligned16(cosv) && aligned16(sinv), (int)kv};
-  if (dtype == kF32) hipLaunchKernelGGL(fp4_store_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL(fp4_store_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  const StoreArgs a{qkv, q, cosv, sinv, slots, (uint8_t*)k_pages, (uint8_t*)v_pages, stride, q_stride, n, nh, nkv, hd, page, pages,
+                    aligned16(qkv) && (size_t)stride * e % 16 == 0, aligned16(q) && (size_t)q_stride * e % 16 == 0,
+                    aligned16(cosv) && aligned16(sinv), (int)kv, k_units, v_units};
+  const dim3 grid((unsigned)blocks), threads(256);
+#define GB_FP4_STORE(T, PAIRS)                                                                                 \
+  if (each == 4) hipLaunchKernelGGL((fp4_store_kernel<T, PAIRS, 4>), grid, threads, 0, stream, a);               \
+  else hipLaunchKernelGGL((fp4_store_kernel<T, PAIRS, 1>), grid, threads, 0, stream, a);
+  if (dtype == kF32 && pairs) { GB_FP4_STORE(float, true) }
+  else if (dtype == kF32) { GB_FP4_STORE(float, false) }
+  else if (pairs) { GB_FP4_STORE(bf16, true) }
+  else { GB_FP4_STORE(bf16, false) }
   return launched("fp4_store");
 }
 

@@ -74,13 +74,13 @@ __device__ __forceinline__ void terms_of(const Raw<float>& v, bf16x8 (&out)[3]) 
   float x[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(v.w[e / 4][e % 4]);
-  fp4_terms<3>(x, out);
+  fp4_terms(x, out);
 }
 
 // T the rows' type, MT tiles of 8 rows of a, NT of 8 rows of W (with silu every other one of the up half), W waves, U blocks of 32 numbers of
 // k that a lane asks for at once
 template <typename T, int MT, int NT, int W, int U>
-__global__ __launch_bounds__(W * kWave) void fp4_lines_kernel(GemmArgs a) {
+__global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(MT * NT * kFp4Terms<T> == 16 ? 2 : 1))) void fp4_lines_kernel(GemmArgs a) {
   constexpr int SP = kFp4Terms<T>;
   const int lane = threadIdx.x % kWave, r = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(W * kWave) void fp4_lines_kernel(GemmArgs a) {
           __builtin_memcpy(&next_x[u][t][w], x[t] + (size_t)c * kFp4Block + 8 * w, sizeof(Raw<T>));
     }
   };
-  const int first = blockIdx.y * a.turns, turns = (a.blocks + 8 * U * W - 1) / (8 * U * W), end = min(turns, first + a.turns);
+  const int first = blockIdx.y * a.turns, turns = (a.blocks - 8 * U * wave + 8 * U * W - 1) / (8 * U * W), end = min(turns, first + a.turns);   // this wave's
   // (the last turn stands by itself: a load behind a branch would be waited for together with all others)
   auto turn = [&](int i, auto last) {
     u32x4 now[U][NT];
@@ -162,9 +162,11 @@ __global__ __launch_bounds__(W * kWave) void fp4_lines_kernel(GemmArgs a) {
         }
       }
   };
-  fetch(first);
-  for (int i = first; i + 1 < end; ++i) turn(i, std::false_type{});
-  turn(end - 1, std::true_type{});
+  if (first < end) {
+    fetch(first);
+    for (int i = first; i + 1 < end; ++i) turn(i, std::false_type{});
+    turn(end - 1, std::true_type{});
+  }
 
   __shared__ f32x4 part[W][NT * MT][kWave];
 #pragma unroll

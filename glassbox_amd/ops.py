@@ -2599,17 +2599,9 @@ def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
                 raise KernelError(f"{what}: operands must be on the current GPU")
 
 
-def _end(t: torch.Tensor, at: int) -> int:
-    """Where the memory of a tensor that begins at ``at`` ends."""
-    return at + (1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else at
-
-
-def _apart(a: torch.Tensor, b: torch.Tensor, what: str, same: bool = False) -> None:
-    """The two share no memory; with ``same`` they may be rows at the same places."""
-    a0, b0 = a.data_ptr(), b.data_ptr()
-    if _end(a, a0) > b0 if a0 < b0 else _end(b, b0) > a0:
-        if not (same and a0 == b0 and a.stride() == b.stride()):
-            raise KernelError(what)
+def _apart(a0: int, a_rows: int, a_bytes: int, a_step: int, b0: int, b_rows: int, b_bytes: int, b_step: int) -> bool:
+    """Whether two arrays of rows, each from an address on, of so many bytes and as many apart, share no memory."""
+    return a0 + (a_rows - 1) * a_step + a_bytes <= b0 if a0 < b0 else b0 + (b_rows - 1) * b_step + b_bytes <= a0
 
 
 def fp4_scale_bytes(columns: int) -> int:
@@ -2673,11 +2665,13 @@ def fp4_store(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torc
         q_stride = _rows(q, "q")
         if q.dtype != qkv.dtype or q.shape != (n, n_heads * head_dim):
             raise KernelError(f"fp4_store: q must be [{n}, {n_heads * head_dim}] of the rows' type")
-        _apart(q, qkv, "fp4_store: q lies over other columns of the rows", same=True)
     dtype = dtype_code(qkv)
+    at, q_at, e = qkv.data_ptr(), q.data_ptr(), 4 if dtype == F32 else 2
+    if not (at == q_at and stride == q_stride) and n and n_heads and not _apart(q_at, n, n_heads * head_dim * e, q_stride * e, at, n, given * e, stride * e):
+        raise KernelError("fp4_store: q lies over other columns of the rows")
     _here("fp4_store", qkv, cos, sin, slots, k_pages, v_pages, q)
     lib = _lib("fp4_cache")
-    _launch(lib, lib.gb_fp4_store, qkv.data_ptr(), dtype, stride, q.data_ptr(), q_stride, cos_at, sin_at, slots_at, k_at, v_at, n, n_heads,
+    _launch(lib, lib.gb_fp4_store, at, dtype, stride, q_at, q_stride, cos_at, sin_at, slots_at, k_at, v_at, n, n_heads,
             n_kv_heads, head_dim, page_size, pages, _stream())
 
 
@@ -2689,11 +2683,13 @@ def fp4_load(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     _i32(slots, "slots", n)
     if k.dtype != v.dtype or k.shape != (n, nkv * hd) or v.shape != (n, nkv * hd):
         raise KernelError(f"fp4_load: k and v must be [{n}, {nkv * hd}] of one type")
-    _apart(k, v, "fp4_load: k and v share memory")
     dtype, k_stride, v_stride = dtype_code(k), _rows(k, "k"), _rows(v, "v")
+    k_to, v_to, e = k.data_ptr(), v.data_ptr(), 4 if dtype == F32 else 2
+    if n and not _apart(k_to, n, nkv * hd * e, k_stride * e, v_to, n, nkv * hd * e, v_stride * e):
+        raise KernelError("fp4_load: k and v share memory")
     _here("fp4_load", slots, k_pages, v_pages, k, v)
     lib = _lib("fp4_cache")
-    _launch(lib, lib.gb_fp4_load, slots.data_ptr(), k_at, v_at, k.data_ptr(), k_stride, v.data_ptr(), v_stride, dtype, n, nkv, hd, page_size,
+    _launch(lib, lib.gb_fp4_load, slots.data_ptr(), k_at, v_at, k_to, k_stride, v_to, v_stride, dtype, n, nkv, hd, page_size,
             pages, _stream())
 
 
@@ -2735,12 +2731,14 @@ def fp4_attention(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_l
     window, max_q_len, max_context = int(window), int(max_q_len), int(max_context)
     if not (0 <= window < 1 << 31 and 0 <= max_q_len < 1 << 31 and 0 <= max_context < 1 << 31):
         raise KernelError("fp4_attention: a window, a number of rows or a context below 0 or beyond 32 bits")
-    _apart(q, out, "fp4_attention: out lies over other rows of q", same=True)
+    dtype, n = dtype_code(q), shape[0]
+    at, to, e = q.data_ptr(), out.data_ptr(), 4 if dtype == F32 else 2
+    if not (at == to and q_stride == out_stride) and n and not _apart(at, n, shape[1] * e, q_stride * e, to, n, shape[1] * e, out_stride * e):
+        raise KernelError("fp4_attention: out lies over other rows of q")
     ws_at, ws_floats = _fp4_workspace(workspace, "fp4_attention")
-    dtype = dtype_code(q)
     _here("fp4_attention", q, out, q_start, q_len, pos0, tables, k_pages, v_pages, workspace)
     lib = _lib("fp4_attention")
-    _launch(lib, lib.gb_fp4_attention, q.data_ptr(), q_stride, out.data_ptr(), out_stride, dtype, shape[0], q_start.data_ptr(), q_len.data_ptr(),
+    _launch(lib, lib.gb_fp4_attention, at, q_stride, to, out_stride, dtype, n, q_start.data_ptr(), q_len.data_ptr(),
             pos0.data_ptr(), seqs, max_q_len, max_context, tables.data_ptr(), tables.stride(0), tables_shape[1], k_at, v_at, pages, n_heads, nkv, hd,
             page_size, scale, window, ws_at, ws_floats, _stream())
 
@@ -2825,15 +2823,17 @@ def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool 
         raise KernelError("fp4_gemm: the fused SiLU-multiply takes an even number of rows of w and does not accumulate")
     if accumulate and out.dtype != torch.float32:
         raise KernelError("fp4_gemm: accumulation is into a 32-bit result")
-    _apart(a, out, "fp4_gemm: a and out share memory")
-    ws_at, floats = _fp4_workspace(workspace, "fp4_gemm")
     dtype, out_dtype = dtype_code(a), dtype_code(out)
+    at, to, e, f = a.data_ptr(), out.data_ptr(), 4 if dtype == F32 else 2, 4 if out_dtype == F32 else 2
+    if M and not _apart(at, M, K * e, lda * e, to, M, (N // 2 if silu_mul else N) * f, ldo * f):
+        raise KernelError("fp4_gemm: a and out share memory")
+    ws_at, floats = _fp4_workspace(workspace, "fp4_gemm")
     _here("fp4_gemm", a, w.codes, w.scales, out, workspace)
-    if floats >= N * K // 2 and _fp4_expands(M, N, K, a.dtype, out.dtype, silu_mul) and lda % 8 == 0 and a.data_ptr() % 16 == 0:
+    if floats >= N * K // 2 and _fp4_expands(M, N, K, a.dtype, out.dtype, silu_mul) and lda % 8 == 0 and at % 16 == 0:
         values, rest = workspace[:N * K // 2].view(torch.bfloat16).view(N, K), workspace[N * K // 2:]
         fp4_expand(w, values)
         gemm(a, values, out, accumulate=accumulate, silu_mul=silu_mul, workspace=rest if rest.numel() >= max(1, gemm_split_floats(M, N, K)) else None)
         return
     lib = _lib("fp4_gemm")
-    _launch(lib, lib.gb_fp4_gemm, a.data_ptr(), dtype, lda, c_at, s_at, each, out.data_ptr(), out_dtype, ldo, M, N, K,
+    _launch(lib, lib.gb_fp4_gemm, at, dtype, lda, c_at, s_at, each, to, out_dtype, ldo, M, N, K,
             2 if silu_mul else 1 if accumulate else 0, ws_at, floats, _stream())

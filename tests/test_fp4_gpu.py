@@ -78,7 +78,9 @@ def test_blocks_that_are_not_finite_read_as_nan_and_no_others():
 
 # -------------------------------------------------------------------------------------------------------------- store and load
 STORES = [  # heads, kv heads, head size, page, rows
-    (1, 1, 32, 16, 1), (9, 3, 64, 16, 5), (4, 4, 96, 32, 33), (8, 2, 128, 16, 70), (2, 1, 256, 48, 17), (0, 2, 64, 16, 4), (32, 32, 64, 16, 8)]
+    (1, 1, 32, 16, 1), (9, 3, 64, 16, 5), (4, 4, 96, 32, 33), (8, 2, 128, 16, 70), (2, 1, 256, 48, 17), (0, 2, 64, 16, 4), (32, 32, 64, 16, 8),
+    # many rows: four heads a lane, the last group not full; values in words and, behind slots out of order, in bytes
+    (9, 5, 64, 16, 1400), (6, 3, 96, 32, 900), (3, 2, 128, 16, 2000)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -93,6 +95,9 @@ def test_store_and_load(H, G, D, page, n, dtype, rotate):
     cos, sin = angle.cos().float(), angle.sin().float()
     g = torch.Generator().manual_seed(4)
     slots = torch.randperm(pages * page, generator=g)[:n].int()
+    if n > 100:                                                      # whole pages in no order, and rows out of order among them
+        slots = (torch.randperm(pages, generator=g)[:-(-n // page), None] * page + torch.arange(page)).flatten()[:n].int()
+        slots[500:520] = slots[500:520].flip(0)
     if n > 3:
         slots[1], slots[2] = -1, pages * page                        # rows that are not stored
     k0 = torch.randint(0, 256, blank(pages, G, page, D).shape, generator=g, dtype=torch.uint8)
@@ -102,9 +107,12 @@ def test_store_and_load(H, G, D, page, n, dtype, rotate):
     kc, ks = plain.quantized(k32)
     vc, vs = plain.quantized(heads[:, H + G:])
     want_k, want_v = k0.clone(), v0.clone()
-    for i in range(n):
-        if 0 <= slots[i] < pages * page:
-            plain.put(want_k, want_v, int(slots[i]), kc[i], ks[i], vc[i], vs[i])
+    kept_rows = [i for i in range(n) if 0 <= slots[i] < pages * page]
+    for i in kept_rows:
+        plain.put(want_k, want_v, int(slots[i]), kc[i], ks[i], vc[i], vs[i])
+    want_k_rows, want_v_rows = torch.full((2, n, G * D), 9.0, dtype=torch.float64)
+    want_k_rows[kept_rows] = plain.values(kc, ks).flatten(1)[kept_rows]
+    want_v_rows[kept_rows] = plain.values(vc, vs).flatten(1)[kept_rows]
     q32 = plain.turned(heads[:, :H], cos, sin) if rotate else heads[:, :H].float()
     want_q = q32.to(dtype).reshape(n, H * D)
     angles = (cos.to(DEV), sin.to(DEV)) if rotate else (None, None)
@@ -125,12 +133,7 @@ def test_store_and_load(H, G, D, page, n, dtype, rotate):
             k = torch.full((n, G * D + 3), 9.0, dtype=dtype, device=DEV)[:, :G * D]
             v = torch.full((n, G * D), 9.0, dtype=dtype, device=DEV)
             ops.fp4_load(slots.to(DEV), kp, vp, k, v)
-            for i in range(n):
-                if 0 <= slots[i] < pages * page:
-                    assert torch.equal(k[i].cpu().double(), plain.values(kc[i], ks[i]).flatten())
-                    assert torch.equal(v[i].cpu().double(), plain.values(vc[i], vs[i]).flatten())
-                else:
-                    assert (k[i] == 9).all() and (v[i] == 9).all()
+            assert torch.equal(k.cpu().double(), want_k_rows) and torch.equal(v.cpu().double(), want_v_rows)
 
 
 def test_store_without_rows():
