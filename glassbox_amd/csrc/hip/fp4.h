@@ -37,8 +37,10 @@ __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t largest) {
   const int b = e - 2 + ((largest & 0x7fffffu) > 0x600000u ? 1 : 0);
   return (uint32_t)(b < 2 ? 2 : b > 252 ? 252 : b);
 }
-// 2^(b - 127) as the conversions take it: they read the exponent's bits alone, and those of 255 make NaN
+// 2^(b - 127) as the conversions take it: they read the exponent's bits alone, whatever stands in the others, and those of 255 make NaN
 __device__ __forceinline__ float fp4_unit(uint32_t b) { return __uint_as_float(b << 23); }
+// of byte i of a word
+__device__ __forceinline__ float fp4_unit_of(uint32_t w, int i) { return __uint_as_float(i < 3 ? w << (23 - 8 * i) : w >> 1); }
 
 // eight numbers to a word, number i in bits 4i..4i+3: divided by the unit, to the nearest, ties to even, at most 6
 __device__ __forceinline__ uint32_t fp4_pack8(const float (&x)[8], float unit) {

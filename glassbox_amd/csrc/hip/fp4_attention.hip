@@ -83,13 +83,346 @@ template <typename T> __device__ __forceinline__ void store4(T* p, bool wide, co
   for (int i = 0; i < 4; ++i) p[i] = (T)x[i];
 }
 
-// T the rows' type, NB blocks a head, R column tiles a wave, W waves, COLS: the waves have columns of their own.  (Two waves a SIMD at least
-// where they do: without the bound 2,048 rows of 32 heads of 128 take 108 us, with it 84.)
-template <typename T, int NB, int R, int W, bool COLS>
-__global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(COLS && NB <= 4 ? 2 : 1))) void fp4_attend_kernel(AttendArgs a) {
+// ---- what both kernels do ------------------------------------------------------------------------------------------------------
+// the page numbers of 16 tokens of keys and 16 of values of a lane, and where in their pages these begin
+struct Places {
+  int kp, vp, koff, voff;
+};
+__device__ __forceinline__ Places look_up(const AttendArgs& a, const int32_t* table, int kt, int vt) {
+  const int ki = a.page_shift >= 0 ? kt >> a.page_shift : kt / a.page, vi = a.page_shift >= 0 ? vt >> a.page_shift : vt / a.page;
+  const int k0 = table[min(ki, a.table_cols - 1)], v0 = table[min(vi, a.table_cols - 1)];
+  return {ki < a.table_cols ? k0 : -1, vi < a.table_cols ? v0 : -1, kt - ki * a.page, vt - vi * a.page};
+}
+// a page of the pool; page 0 in the place of any other number, which is not read
+__device__ __forceinline__ bool known_page(const AttendArgs& a, int page) { return (unsigned)page < (unsigned)a.pages; }
+__device__ __forceinline__ size_t page_at(const AttendArgs& a, int page, int kvh, size_t head_bytes) {
+  return ((size_t)(known_page(a, page) ? page : 0) * a.nkv + kvh) * head_bytes;
+}
+
+// the query of a column, its channels as the lanes take those of the keys
+template <typename T, int NB> __device__ __forceinline__ void load_query(const T* row, int g, bool wide, bf16x8 (&qf)[kFp4Terms<T>][NB]) {
   using U = Units<NB>;
-  constexpr int D = NB * kFp4Block, SP = kFp4Terms<T>, C = 16 * R;
-  static_assert(COLS || R == 1, "waves that share their columns hold one tile of them");
+#pragma unroll
+  for (int i = 0; i < U::kCount; ++i)
+#pragma unroll
+    for (int w = 0; w < U::kWords; ++w) {
+      float x[8];
+      load8(row + (g + 4 * i) * U::kChannels + 8 * w, wide, x);
+      bf16x8 terms[kFp4Terms<T>];
+      fp4_terms(x, terms);
+#pragma unroll
+      for (int p = 0; p < kFp4Terms<T>; ++p) qf[p][i * U::kWords + w] = terms[p];
+    }
+}
+
+// Scores of 16 keys from `key` on that the column does not see become minus infinity; the bits of those it sees.
+__device__ __forceinline__ uint32_t mask_scores(f32x4 (&sc)[4], int key, bool known, int from, int pos, int end) {
+  uint32_t seen = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int k = key + 4 * j + x;
+      const bool in = known && k >= from && k <= pos && k < end;
+      seen |= in ? 1u << (4 * j + x) : 0u;
+      sc[j][x] = in ? sc[j][x] : -__builtin_inff();
+    }
+  return seen;
+}
+
+// One step of the running softmax of a column (this lane's 16 keys of 64): probabilities as the product's operand, sums rescaled where
+// the maximum grows.
+template <int SP, int NB>
+__device__ __forceinline__ void soften(const f32x4 (&sc)[4], float scale, float& m, float& l, f32x4 (&o)[2 * NB], bf16x8 (&pf)[SP][2]) {
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) top = fmaxf(top, sc[j][x]);
+  const float now = fmaxf(m, quads_max(top) * scale);   // (the scale is positive)
+  if (__any(now > m)) {
+    const float shrink = now > m ? __builtin_amdgcn_exp2f(m - now) : 1.f;
+    m = now;
+    l *= shrink;
+#pragma unroll
+    for (int b = 0; b < 2 * NB; ++b)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[b][x] *= shrink;
+  }
+  const float sub = m == -__builtin_inff() ? 0.f : m;
+  float p[16], sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      p[4 * j + x] = __builtin_amdgcn_exp2f(fmaf(sc[j][x], scale, -sub));
+      sum += p[4 * j + x];
+    }
+  l += sum;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = p[8 * c + e];
+    bf16x8 terms[SP];
+    fp4_terms(x, terms);
+#pragma unroll
+    for (int q = 0; q < SP; ++q) pf[q][c] = terms[q];
+  }
+}
+
+// Eight tokens of a byte row of values: the operands of channels i (low) and i + 16.
+__device__ __forceinline__ void values8(uint32_t w0, uint32_t w1, uint32_t s0, uint32_t s1, bf16x8& low, bf16x8& high) {
+  uint32_t two[8];   // both channels of a token
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t w = e < 4 ? w0 : w1;
+    const float unit = fp4_unit_of(e < 4 ? s0 : s1, e % 4);
+    bf16x2 y;
+    if (e % 4 == 0) y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 0);
+    else if (e % 4 == 1) y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 1);
+    else if (e % 4 == 2) y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 2);
+    else y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 3);
+    two[e] = __builtin_bit_cast(uint32_t, y);
+  }
+  u32x4 a, b;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    a[e] = __builtin_amdgcn_perm(two[2 * e + 1], two[2 * e], 0x05040100u);
+    b[e] = __builtin_amdgcn_perm(two[2 * e + 1], two[2 * e], 0x07060302u);
+  }
+  low = __builtin_bit_cast(bf16x8, a);
+  high = __builtin_bit_cast(bf16x8, b);
+}
+
+// A probability of zero times a value that is not finite is not zero: the blocks that are marked so take part as finite ones, and are
+// counted for the columns that see them, which become NaN.  Scales and seen keys of eight tokens.
+__device__ __forceinline__ void count_bad(uint32_t s0, uint32_t s1, uint32_t seen, f32x4& count) {
+  bf16x8 is, sees;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    is[e] = ((e < 4 ? s0 : s1) >> (8 * (e % 4)) & 255u) == kFp4BadScale ? (bf16)1.f : (bf16)0.f;
+    sees[e] = seen >> e & 1u ? (bf16)1.f : (bf16)0.f;
+  }
+  count = mfma(is, sees, count);
+}
+
+// 0xff in each byte of a word of four tokens from `key` on that some column sees
+__device__ __forceinline__ uint32_t kept_bytes(int key, int from, int to) {
+  uint32_t keep = 0;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) keep |= key + x >= from && key + x < to ? 0xffu << (8 * x) : 0u;
+  return keep;
+}
+
+// a tile of 64 keys and values as a lane takes them from memory
+template <int NB> struct Tile {
+  uint32_t kw[4][NB], ks[Units<NB>::kCount];
+  u32x4 vw[NB], vs[NB];
+};
+template <int NB> __device__ __forceinline__ void load_tile(const AttendArgs& a, const Places& at, int kvh, int r, int g, Tile<NB>& t) {
+  using U = Units<NB>;
+  const size_t block = fp4_block_bytes(a.page), head_bytes = block * NB;
+  const uint8_t* kb = a.k + page_at(a, at.kp, kvh, head_bytes);
+  const uint8_t* vb = a.v + page_at(a, at.vp, kvh, head_bytes);
+  const int kslot = r & 3;
+#pragma unroll
+  for (int i = 0; i < U::kCount; ++i) {
+    const int u = g + 4 * i;
+    const uint8_t* base = kb + (size_t)(u * U::kChannels / kFp4Block) * block;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      __builtin_memcpy(&t.kw[j][i * U::kWords], __builtin_assume_aligned(base + (at.koff + 4 * j + kslot) * 16 + u * U::kChannels % kFp4Block / 2, 4 * U::kWords),
+                       4 * U::kWords);
+    t.ks[i] = *reinterpret_cast<const uint32_t*>(base + 16 * a.page + at.koff + 4 * kslot);
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    t.vw[b] = *reinterpret_cast<const u32x4*>(vb + (size_t)b * block + (size_t)r * a.page + at.voff);
+    t.vs[b] = *reinterpret_cast<const u32x4*>(vb + (size_t)b * block + (size_t)16 * a.page + at.voff);
+  }
+}
+
+// R tiles of 16 columns over a tile of keys: their scores, the step of their softmax, their sums.  first, last: the columns' positions;
+// [lo, end): keys that some column may see.
+template <typename T, int NB, int R> struct Columns {
+  static constexpr int SP = kFp4Terms<T>;
+  bf16x8 qf[R][SP][NB];
+  f32x4 o[R][2 * NB];
+  float m[R], l[R];
+  int pos[R], from[R];   // a column sees the keys from .. pos
+
+  __device__ __forceinline__ void begin(const AttendArgs& a, int q_start, int pos0, int kvh, int c0, int cols, int r, int g) {
+#pragma unroll
+    for (int t = 0; t < R; ++t) {
+      const int c = min(c0 + 16 * t + r, cols - 1);
+      pos[t] = pos0 + c / a.rep;
+      from[t] = a.window > 0 ? pos[t] - a.window + 1 : 0;
+      load_query<T, NB>((const T*)a.q + (size_t)(q_start + c / a.rep) * a.q_stride + (size_t)(kvh * a.rep + c % a.rep) * (NB * kFp4Block), g, a.q_wide, qf[t]);
+      m[t] = -__builtin_inff();
+      l[t] = 0.f;
+#pragma unroll
+      for (int b = 0; b < 2 * NB; ++b) o[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  __device__ __forceinline__ void take(const AttendArgs& a, Tile<NB>& w, int t0, bool known, int first, int last, int lo, int end, int g) {
+    const int key = t0 + 16 * g;   // this lane's 16
+    f32x4 sc[R][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int t = 0; t < R; ++t) sc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const bf16x8 kf = fp4_unpack8(w.kw[j][i], fp4_unit_of(w.ks[i / Units<NB>::kWords], j));
+#pragma unroll
+        for (int t = 0; t < R; ++t)
+#pragma unroll
+          for (int p = 0; p < SP; ++p) sc[t][j] = mfma(kf, qf[t][p][i], sc[t][j]);
+      }
+    }
+    // tiles that some column sees in part
+    const bool whole = t0 + kTile <= first + 1 && t0 + kTile <= end && (a.window <= 0 || t0 > last - a.window) && __all(known);
+    bool bad = false;   // a value that may be behind a mask stands in a block that is not finite
+    uint32_t seen[R];
+#pragma unroll
+    for (int t = 0; t < R; ++t) seen[t] = 0xffffu;
+    if (!whole) {
+#pragma unroll
+      for (int t = 0; t < R; ++t) seen[t] = mask_scores(sc[t], key, known, from[t], pos[t], end);
+      // (what no column sees, the rest of a last page among it, may be anything: its scales become the smallest)
+      uint32_t any = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t keep = known ? kept_bytes(key + 4 * e, lo, end) : 0u;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          w.vs[b][e] &= keep;
+          any |= bytes_255(w.vs[b][e]);
+        }
+      }
+      bad = __any(any != 0);
+    }
+    bf16x8 pf[R][SP][2];
+#pragma unroll
+    for (int t = 0; t < R; ++t) soften<SP, NB>(sc[t], a.scale, m[t], l[t], o[t], pf[t]);
+    if (__builtin_expect(bad, 0)) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int t = 0; t < R; ++t) {
+          f32x4 count = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) count_bad(w.vs[b][2 * c], w.vs[b][2 * c + 1], seen[t] >> (8 * c), count);
+          if (count[0] > 0.f) o[t][2 * b] = o[t][2 * b + 1] = f32x4{} + __builtin_nanf("");
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.vs[b][e] &= ~bytes_255(w.vs[b][e]);   // 255 becomes 127
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        bf16x8 low, high;
+        values8(w.vw[b][2 * c], w.vw[b][2 * c + 1], w.vs[b][2 * c], w.vs[b][2 * c + 1], low, high);
+#pragma unroll
+        for (int t = 0; t < R; ++t)
+#pragma unroll
+          for (int p = 0; p < SP; ++p) {
+            o[t][2 * b] = mfma(low, pf[t][p][c], o[t][2 * b]);
+            o[t][2 * b + 1] = mfma(high, pf[t][p][c], o[t][2 * b + 1]);
+          }
+      }
+  }
+};
+
+// Waves a SIMD holds at least: what just fits the registers.  (Without the bound a few more registers cost a wave: 40 requests of 8,000 keys 63 us, with
+// it 59.)
+template <typename T, int NB, int R> constexpr int least_waves = NB > 4 ? 1 : std::is_same_v<T, float> || R > 1 ? 2 : NB > 2 ? 3 : 4;
+
+// Few columns: the waves of a workgroup share out the tiles of keys.  T the rows' type, NB blocks a head, W waves.  Bound by memory: 64 requests of
+// 4,096 keys, 32 heads of 64, 119 us for 571 MB (4.8 TB/s); 64 of 4,000, 8 kv heads of 128, 59 us (4.7 TB/s).
+template <typename T, int NB, int W>
+__global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least_waves<T, NB, 1>))) void fp4_attend_keys_kernel(AttendArgs a) {
+  constexpr int D = NB * kFp4Block;
+  const int lane = threadIdx.x % kWave, r = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  int id = blockIdx.x;
+  const int kvh = id % a.nkv;
+  id /= a.nkv;
+  const int c0 = id % a.col_tiles * 16;
+  id /= a.col_tiles;
+  const int split = id % a.splits, s = id / a.splits;
+
+  const int q_start = a.q_start[s], pos0 = a.pos0[s];
+  const int cols = q_start < 0 ? 0 : min(min(a.q_len[s], a.max_q), a.n - q_start) * a.rep;
+  if (c0 >= cols) return;   // (the whole workgroup)
+  const int first = pos0 + c0 / a.rep, last = pos0 + min(cols - 1, c0 + 15) / a.rep;   // positions of the columns
+  const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0, begin = (lo & ~(kTile - 1)) + split * a.chunk;
+  const int end = min(min(last + 1, a.table_cols * a.page), begin + a.chunk);
+
+  // the numbers of a tile's pages are asked for a tile ahead, those of the first before the queries
+  const int32_t* table = a.tables + (size_t)s * a.table_stride;
+  const int start = begin + wave * kTile;
+  Places at = look_up(a, table, start + 16 * (r >> 2), start + 16 * g);
+  Columns<T, NB, 1> columns;
+  columns.begin(a, q_start, pos0, kvh, c0, cols, r, g);
+  for (int t0 = start; t0 < end; t0 += W * kTile) {
+    const bool known = known_page(a, at.vp);
+    Tile<NB> tile;
+    load_tile(a, at, kvh, r, g, tile);
+    __builtin_amdgcn_sched_barrier(0);   // (all of a tile is asked for before anything is computed: 62.8 us without, 61.8 with)
+    at = look_up(a, table, t0 + W * kTile + 16 * (r >> 2), t0 + W * kTile + 16 * g);
+    columns.take(a, tile, t0, known, first, last, lo, end, g);
+  }
+
+  constexpr int kPad = 4, kThreads = W * 4, kEach = D / kThreads;   // threads a column, channels a thread
+  __shared__ float so[W][16][D + kPad];
+  __shared__ float sm[W][16], sl[W][16];
+  const float l = quads_sum(columns.l[0]);
+  if (g == 0) sm[wave][r] = columns.m[0], sl[wave][r] = l;
+#pragma unroll
+  for (int b = 0; b < 2 * NB; ++b) *reinterpret_cast<f32x4*>(&so[wave][r][16 * b + 4 * g]) = columns.o[0][b];
+  __syncthreads();
+  const int column = threadIdx.x / kThreads, part = threadIdx.x % kThreads, c = c0 + column;
+  if (c >= cols) return;
+  float top = sm[0][column], sum = 0.f, weight[W];
+#pragma unroll
+  for (int w = 1; w < W; ++w) top = fmaxf(top, sm[w][column]);
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    weight[w] = sm[w][column] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sm[w][column] - top);
+    sum += weight[w] * sl[w][column];
+  }
+  float x[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    x[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) x[e] = fmaf(weight[w], so[w][column][part * kEach + e], x[e]);
+  }
+  if (a.splits > 1) {
+    const size_t to = (((size_t)s * a.nkv + kvh) * a.max_q * a.rep + c) * a.splits + split;
+    if (part == 0) a.ml[to] = make_float2(top, sum);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) a.acc[to * D + part * kEach + e] = x[e];
+  } else {
+    const float over = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    T* row = (T*)a.out + (size_t)(q_start + c / a.rep) * a.out_stride + (size_t)(kvh * a.rep + c % a.rep) * D;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) row[part * kEach + e] = (T)(x[e] * over);
+  }
+}
+
+// More columns: each of four waves has R tiles of its own and takes all keys.  Bound by the conversions and the softmax: 2,048 rows of 32 heads of
+// 128 in 64 us (the same rows over a bf16 cache in the prefill kernel: 56).  A request's long tiles of columns come first and its short ones
+// behind them in turn, so that compute units of two workgroups have about the same to do: in their order 84.  Making a tile bf16 once for the four waves, through LDS, took 95: the barriers cost more than the
+// conversions that they save.
+template <typename T, int NB, int R>
+__global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(least_waves<T, NB, R>))) void fp4_attend_cols_kernel(AttendArgs a) {
+  constexpr int D = NB * kFp4Block, C = 16 * R;
   const int lane = threadIdx.x % kWave, r = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   // kv heads fastest: the workgroups of one request and kv head, which read the same keys, are a multiple of nkv apart and, where
@@ -97,327 +430,50 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(COLS 
   int id = blockIdx.x;
   const int kvh = id % a.nkv;
   id /= a.nkv;
-  const int col_tile = id % a.col_tiles;
+  const int turn = id % a.col_tiles, col_tile = turn < a.col_tiles / 2 ? a.col_tiles - 1 - turn : turn - a.col_tiles / 2;
   id /= a.col_tiles;
   const int split = id % a.splits, s = id / a.splits;
 
   const int q_start = a.q_start[s], pos0 = a.pos0[s];
-  const int q_len = min(min(a.q_len[s], a.max_q), a.n - q_start);
-  const int cols = q_start < 0 ? 0 : q_len * a.rep;
-  const int c0 = (col_tile * (COLS ? W : 1) + (COLS ? wave : 0)) * C;
-  if (c0 >= cols) return;   // (without COLS the whole workgroup)
-  const int first = pos0 + c0 / a.rep, last = pos0 + min(cols - 1, c0 + C - 1) / a.rep;   // positions of this wave's columns
-  const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-  const int begin = (lo & ~(kTile - 1)) + split * a.chunk;
+  const int cols = q_start < 0 ? 0 : min(min(a.q_len[s], a.max_q), a.n - q_start) * a.rep;
+  const int c0 = (col_tile * 4 + wave) * C;
+  if (c0 >= cols) return;   // (the wave: there is no barrier)
+  const int first = pos0 + c0 / a.rep, last = pos0 + min(cols - 1, c0 + C - 1) / a.rep;   // positions of the wave's columns
+  const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0, begin = (lo & ~(kTile - 1)) + split * a.chunk;
   const int end = min(min(last + 1, a.table_cols * a.page), begin + a.chunk);
 
-  // The numbers of a tile's pages are asked for a tile ahead, those of the first before the queries.  What is no page of the pool is not
-  // read (page 0 is, in its place), its keys are not seen.
   const int32_t* table = a.tables + (size_t)s * a.table_stride;
-  const int start = begin + (COLS ? 0 : wave * kTile), stride = COLS ? kTile : W * kTile;
-  int kp, vp, koff, voff;   // of this lane's keys, 16 tokens all of which one page holds, and of its values
-  auto look_up = [&](int t0) {
-    const int kt = t0 + 16 * (r >> 2), vt = t0 + 16 * g;
-    const int ki = a.page_shift >= 0 ? kt >> a.page_shift : kt / a.page, vi = a.page_shift >= 0 ? vt >> a.page_shift : vt / a.page;
-    koff = kt - ki * a.page;
-    voff = vt - vi * a.page;
-    const int k0 = table[min(ki, a.table_cols - 1)], v0 = table[min(vi, a.table_cols - 1)];
-    kp = ki < a.table_cols ? k0 : -1;
-    vp = vi < a.table_cols ? v0 : -1;
-  };
-  look_up(start);
+  Places at = look_up(a, table, begin + 16 * (r >> 2), begin + 16 * g);
+  Columns<T, NB, R> columns;
+  columns.begin(a, q_start, pos0, kvh, c0, cols, r, g);
+  for (int t0 = begin; t0 < end; t0 += kTile) {
+    const bool known = known_page(a, at.vp);
+    Tile<NB> tile;
+    load_tile(a, at, kvh, r, g, tile);
+    at = look_up(a, table, t0 + kTile + 16 * (r >> 2), t0 + kTile + 16 * g);
+    columns.take(a, tile, t0, known, first, last, lo, end, g);
+  }
 
-  int pos[R], from[R];   // a column sees the keys from .. pos
-  bool own[R];
-  bf16x8 qf[R][SP][NB];
 #pragma unroll
   for (int t = 0; t < R; ++t) {
+    const float sum = quads_sum(columns.l[t]);
     const int c = c0 + 16 * t + r;
-    own[t] = c < cols;
-    const int cc = own[t] ? c : cols - 1;
-    pos[t] = pos0 + cc / a.rep;
-    from[t] = a.window > 0 ? pos[t] - a.window + 1 : 0;
-    const T* row = (const T*)a.q + (size_t)(q_start + cc / a.rep) * a.q_stride + (size_t)(kvh * a.rep + cc % a.rep) * D;
-#pragma unroll
-    for (int i = 0; i < U::kCount; ++i)
-#pragma unroll
-      for (int w = 0; w < U::kWords; ++w) {
-        float x[8];
-        load8(row + (g + 4 * i) * U::kChannels + 8 * w, a.q_wide, x);
-        bf16x8 terms[SP];
-        fp4_terms(x, terms);
-#pragma unroll
-        for (int p = 0; p < SP; ++p) qf[t][p][i * U::kWords + w] = terms[p];
-      }
-  }
-
-  f32x4 o[R][2 * NB];
-  float m[R], l[R];
-#pragma unroll
-  for (int t = 0; t < R; ++t) {
-    m[t] = -__builtin_inff();
-    l[t] = 0.f;
-#pragma unroll
-    for (int b = 0; b < 2 * NB; ++b) o[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  const size_t block = fp4_block_bytes(a.page), head_bytes = block * NB;
-  const int kslot = r & 3;
-  for (int t0 = start; t0 < end; t0 += stride) {
-    const int vt = t0 + 16 * g;
-    const bool known = (unsigned)vp < (unsigned)a.pages;
-    const uint8_t* kb = a.k + ((size_t)((unsigned)kp < (unsigned)a.pages ? kp : 0) * a.nkv + kvh) * head_bytes;
-    const uint8_t* vb = a.v + ((size_t)(known ? vp : 0) * a.nkv + kvh) * head_bytes;
-
-    uint32_t kw[4][NB], ks[U::kCount];
-    u32x4 vw[NB], vs[NB];
-#pragma unroll
-    for (int i = 0; i < U::kCount; ++i) {
-      const int u = g + 4 * i, b = u * U::kChannels / kFp4Block, in = u * U::kChannels % kFp4Block / 2;
-      const uint8_t* base = kb + (size_t)b * block;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint8_t* p = base + (koff + 4 * j + kslot) * 16 + in;
-        if constexpr (U::kWords == 4) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) kw[j][4 * i + e] = w[e];
-        } else if constexpr (U::kWords == 2) {
-          const u32x2 w = *reinterpret_cast<const u32x2*>(p);
-          kw[j][2 * i] = w[0], kw[j][2 * i + 1] = w[1];
-        } else {
-          kw[j][i] = *reinterpret_cast<const uint32_t*>(p);
-        }
-      }
-      ks[i] = *reinterpret_cast<const uint32_t*>(base + 16 * a.page + koff + 4 * kslot);
-    }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      vw[b] = *reinterpret_cast<const u32x4*>(vb + (size_t)b * block + (size_t)r * a.page + voff);
-      vs[b] = *reinterpret_cast<const u32x4*>(vb + (size_t)b * block + (size_t)16 * a.page + voff);
-    }
-    look_up(t0 + stride);
-
-    f32x4 sc[R][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int t = 0; t < R; ++t) sc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < U::kCount; ++i)
-#pragma unroll
-        for (int w = 0; w < U::kWords; ++w) {
-          const bf16x8 kf = fp4_unpack8(kw[j][i * U::kWords + w], fp4_unit(ks[i] >> (8 * j) & 255u));
-#pragma unroll
-          for (int t = 0; t < R; ++t)
-#pragma unroll
-            for (int p = 0; p < SP; ++p) sc[t][j] = mfma(kf, qf[t][p][i * U::kWords + w], sc[t][j]);
-        }
-    }
-
-    // tiles that some column sees in part
-    const bool whole = t0 + kTile <= first + 1 && t0 + kTile <= end && (a.window <= 0 || t0 > last - a.window) && __all(known);
-    bool bad = false;      // a value of this tile that may be behind a mask stands in a block that is not finite
-    uint32_t seen[R];      // of this lane's 16 keys
-#pragma unroll
-    for (int t = 0; t < R; ++t) seen[t] = 0xffffu;
-    if (!whole) {
-#pragma unroll
-      for (int t = 0; t < R; ++t) {
-        seen[t] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int key = vt + 4 * j + x;
-            const bool in = known && key <= pos[t] && key >= from[t] && key < end;
-            seen[t] |= in ? 1u << (4 * j + x) : 0u;
-            sc[t][j][x] = in ? sc[t][j][x] : -__builtin_inff();
-          }
-      }
-      // (what no column sees, the rest of a last page among it, may be anything: its scales become the smallest)
-      uint32_t any = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t keep = 0;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int key = vt + 4 * e + x;
-          keep |= known && key >= lo && key <= last && key < end ? 0xffu << (8 * x) : 0u;
-        }
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          vs[b][e] &= keep;
-          any |= bytes_255(vs[b][e]);
-        }
-      }
-      bad = __any(any != 0);
-    }
-
-    bf16x8 pf[R][SP][2];
-#pragma unroll
-    for (int t = 0; t < R; ++t) {
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) top = fmaxf(top, sc[t][j][x]);
-      // scale is positive or the maximum is of the scaled scores: see below
-      top = quads_max(top) * a.scale;
-      const float now = fmaxf(m[t], top);
-      if (__any(now > m[t])) {
-        const float shrink = now > m[t] ? __builtin_amdgcn_exp2f(m[t] - now) : 1.f;
-        m[t] = now;
-        l[t] *= shrink;
-#pragma unroll
-        for (int b = 0; b < 2 * NB; ++b)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) o[t][b][x] *= shrink;
-      }
-      const float sub = m[t] == -__builtin_inff() ? 0.f : m[t];
-      float p[16], sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          p[4 * j + x] = __builtin_amdgcn_exp2f(fmaf(sc[t][j][x], a.scale, -sub));
-          sum += p[4 * j + x];
-        }
-      l[t] += sum;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = p[8 * c + e];
-        bf16x8 terms[SP];
-        fp4_terms(x, terms);
-#pragma unroll
-        for (int q = 0; q < SP; ++q) pf[t][q][c] = terms[q];
-      }
-    }
-
-    if (__builtin_expect(bad, 0)) {
-      // a probability of zero times a value that is not finite is not zero: such blocks are counted for the columns that see
-      // them, which become NaN, and take part as finite ones
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        f32x4 count[R];
-#pragma unroll
-        for (int t = 0; t < R; ++t) count[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          bf16x8 is;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) is[e] = (vs[b][2 * c + e / 4] >> (8 * (e % 4)) & 255u) == kFp4BadScale ? (bf16)1.f : (bf16)0.f;
-#pragma unroll
-          for (int t = 0; t < R; ++t) {
-            bf16x8 sees;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sees[e] = seen[t] >> (8 * c + e) & 1u ? (bf16)1.f : (bf16)0.f;
-            count[t] = mfma(is, sees, count[t]);
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < R; ++t)
-          if (count[t][0] > 0.f) o[t][2 * b] = o[t][2 * b + 1] = f32x4{} + __builtin_nanf("");
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vs[b][e] &= ~bytes_255(vs[b][e]);   // 255 becomes 127
-      }
-    }
-
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t two[8];   // channels r (low) and r + 16 of a token
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float unit = fp4_unit(vs[b][2 * c + e / 4] >> (8 * (e % 4)) & 255u);
-          const uint32_t w = vw[b][2 * c + e / 4];
-          bf16x2 y;
-          if (e % 4 == 0) y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 0);
-          else if (e % 4 == 1) y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 1);
-          else if (e % 4 == 2) y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 2);
-          else y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, unit, 3);
-          two[e] = __builtin_bit_cast(uint32_t, y);
-        }
-        u32x4 low, high;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          low[e] = __builtin_amdgcn_perm(two[2 * e + 1], two[2 * e], 0x05040100u);
-          high[e] = __builtin_amdgcn_perm(two[2 * e + 1], two[2 * e], 0x07060302u);
-        }
-        const bf16x8 vl = __builtin_bit_cast(bf16x8, low), vh = __builtin_bit_cast(bf16x8, high);
-#pragma unroll
-        for (int t = 0; t < R; ++t)
-#pragma unroll
-          for (int p = 0; p < SP; ++p) {
-            o[t][2 * b] = mfma(vl, pf[t][p][c], o[t][2 * b]);
-            o[t][2 * b + 1] = mfma(vh, pf[t][p][c], o[t][2 * b + 1]);
-          }
-      }
-  }
-#pragma unroll
-  for (int t = 0; t < R; ++t) l[t] = quads_sum(l[t]);
-
-  const size_t column0 = ((size_t)s * a.nkv + kvh) * a.max_q * a.rep;   // of the partial results
-  if constexpr (COLS) {
-#pragma unroll
-    for (int t = 0; t < R; ++t) {
-      if (!own[t]) continue;
-      const int c = c0 + 16 * t + r;
-      if (a.splits > 1) {
-        const size_t at = (column0 + c) * a.splits + split;
-        if (g == 0) a.ml[at] = make_float2(m[t], l[t]);
-#pragma unroll
-        for (int b = 0; b < 2 * NB; ++b) *reinterpret_cast<f32x4*>(a.acc + at * D + 16 * b + 4 * g) = o[t][b];
-      } else {
-        const float over = l[t] > 0.f || l[t] != l[t] ? 1.f / l[t] : 0.f;
-        T* row = (T*)a.out + (size_t)(q_start + c / a.rep) * a.out_stride + (size_t)(kvh * a.rep + c % a.rep) * D;
-#pragma unroll
-        for (int b = 0; b < 2 * NB; ++b) {
-          float x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = o[t][b][e] * over;
-          store4<T>(row + 16 * b + 4 * g, a.out_wide, x);
-        }
-      }
-    }
-  } else {
-    constexpr int kPad = 4, kThreads = W * 4, kEach = D / kThreads;   // threads a column, channels a thread
-    __shared__ float so[W][16][D + kPad];
-    __shared__ float sm[W][16], sl[W][16];
-    if (g == 0) sm[wave][r] = m[0], sl[wave][r] = l[0];
-#pragma unroll
-    for (int b = 0; b < 2 * NB; ++b) *reinterpret_cast<f32x4*>(&so[wave][r][16 * b + 4 * g]) = o[0][b];
-    __syncthreads();
-    const int column = threadIdx.x / kThreads, part = threadIdx.x % kThreads, c = c0 + column;
-    if (c >= cols) return;
-    float top = sm[0][column], sum = 0.f, weight[W];
-#pragma unroll
-    for (int w = 1; w < W; ++w) top = fmaxf(top, sm[w][column]);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      weight[w] = sm[w][column] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sm[w][column] - top);
-      sum += weight[w] * sl[w][column];
-    }
-    float x[kEach];
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      x[e] = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) x[e] = fmaf(weight[w], so[w][column][part * kEach + e], x[e]);
-    }
+    if (c >= cols) continue;
     if (a.splits > 1) {
-      const size_t at = (column0 + c) * a.splits + split;
-      if (part == 0) a.ml[at] = make_float2(top, sum);
+      const size_t to = (((size_t)s * a.nkv + kvh) * a.max_q * a.rep + c) * a.splits + split;
+      if (g == 0) a.ml[to] = make_float2(columns.m[t], sum);
 #pragma unroll
-      for (int e = 0; e < kEach; ++e) a.acc[at * D + part * kEach + e] = x[e];
+      for (int b = 0; b < 2 * NB; ++b) *reinterpret_cast<f32x4*>(a.acc + to * D + 16 * b + 4 * g) = columns.o[t][b];
     } else {
       const float over = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
       T* row = (T*)a.out + (size_t)(q_start + c / a.rep) * a.out_stride + (size_t)(kvh * a.rep + c % a.rep) * D;
 #pragma unroll
-      for (int e = 0; e < kEach; ++e) row[part * kEach + e] = (T)(x[e] * over);
+      for (int b = 0; b < 2 * NB; ++b) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = columns.o[t][b][e] * over;
+        store4<T>(row + 16 * b + 4 * g, a.out_wide, x);
+      }
     }
   }
 }
@@ -436,12 +492,15 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int columns
   const float sum = wave_sum(weight * ml.y), over = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   constexpr int kEach = (D + kWave - 1) / kWave;
   float x[kEach] = {};
-  // (runs in which a column sees nothing have left zeros)
-#pragma unroll 8
-  for (int i = 0; i < a.splits; ++i) {
-    const float w = __shfl(weight, i, kWave);
+  // (runs in which a column sees nothing have left zeros; what is read again behind the last has no weight)
+  for (int i = 0; i < a.splits; i += 8) {
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) x[e] = fmaf(w, a.acc[((size_t)at * a.splits + i) * D + min(lane + e * kWave, D - 1)], x[e]);
+    for (int k = 0; k < 8; ++k) {
+      const float w = __shfl(weight, i + k, kWave);
+      const float* run = a.acc + ((size_t)at * a.splits + min(i + k, a.splits - 1)) * D;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) x[e] = fmaf(w, run[min(lane + e * kWave, D - 1)], x[e]);
+    }
   }
   T* row = (T*)a.out + (size_t)(q_start + token) * a.out_stride + (size_t)(kvh * a.rep + c % a.rep) * D;
 #pragma unroll
@@ -459,12 +518,13 @@ static Plan plan(int n_seqs, int nkv, int rep, int hd, int max_q, int max_contex
   Plan p;
   const long long columns = (long long)max_q * rep;
   p.cols = columns > 32;
-  // Waves with columns of their own: two tiles of them where there are many and they fit the registers (2,048 rows of 32 heads of 128: 84 us,
-  // one tile 96; 120 rows of 5 requests, 3 heads a kv head: 7.7 and 5.9; 64 rows behind 8,000, 4 a kv head: 37.7 and 36.5).
-  p.r = p.cols && columns >= 1024 && dtype == kBF16 && hd <= 128 ? 2 : 1;
-  const int width = p.cols ? 64 * p.r : 16;
+  // Waves with columns of their own: two tiles of them where there is much to do and they fit the registers (2,048 rows of 32 heads of 128: 64 us,
+  // one tile 89; 131 rows behind 3,900: 29.1 and 30.9; 120 rows of 5 requests, 3 heads a kv head: 7.7 and 5.9).
+  const long long longest = window > 0 ? std::min(max_context, window) : max_context;
+  p.r = p.cols && (columns >= 1024 || (columns >= 128 && longest >= 2048)) && dtype == kBF16 && hd <= 128 ? 2 : 1;
+  const int width = p.cols ? 64 * p.r : 16;   // columns a workgroup
   p.col_tiles = (int)((columns + width - 1) / width);
-  const long long tokens = std::min<long long>(max_q, (16 * p.r - 1) / rep + 2);
+  const long long tokens = std::min<long long>(max_q, (16 * p.r - 1) / rep + 2);   // of a wave's columns
   const long long span = window > 0 ? std::min<long long>(max_context, window + tokens + kTile) : max_context;
   // Runs of a context: about as many workgroups as compute units (half as many again of four waves), none of fewer than 1,024 keys (256).  us:
   // 4 requests of 16,000 keys and 8 kv heads in 8 runs 23.6, in 4 29.6, in 16 28.7; 256 workgroups in one run 18.2, in two 21.9; 131 rows behind
@@ -481,9 +541,9 @@ static Plan plan(int n_seqs, int nkv, int rep, int hd, int max_q, int max_contex
 template <typename T, int NB> static void launch(const Plan& p, const AttendArgs& a, int n_seqs, hipStream_t stream) {
   constexpr int W = NB == 8 ? 4 : 8;   // (the waves' sums of heads of 256 would not fit LDS twice)
   const dim3 grid((unsigned)((long long)n_seqs * a.nkv * p.col_tiles * p.splits));
-  if (!p.cols) hipLaunchKernelGGL((fp4_attend_kernel<T, NB, 1, W, false>), grid, dim3(W * kWave), 0, stream, a);
-  else if (p.r == 1) hipLaunchKernelGGL((fp4_attend_kernel<T, NB, 1, 4, true>), grid, dim3(4 * kWave), 0, stream, a);
-  else if constexpr (std::is_same_v<T, bf16> && NB <= 4) hipLaunchKernelGGL((fp4_attend_kernel<T, NB, 2, 4, true>), grid, dim3(4 * kWave), 0, stream, a);
+  if (!p.cols) hipLaunchKernelGGL((fp4_attend_keys_kernel<T, NB, W>), grid, dim3(W * kWave), 0, stream, a);
+  else if (p.r == 1) hipLaunchKernelGGL((fp4_attend_cols_kernel<T, NB, 1>), grid, dim3(4 * kWave), 0, stream, a);
+  else if constexpr (std::is_same_v<T, bf16> && NB <= 4) hipLaunchKernelGGL((fp4_attend_cols_kernel<T, NB, 2>), grid, dim3(4 * kWave), 0, stream, a);
   if (p.splits > 1) {
     const int columns = n_seqs * a.nkv * a.max_q * a.rep;
     hipLaunchKernelGGL((fp4_join_kernel<T, NB * kFp4Block>), dim3((columns + 3) / 4), dim3(256), 0, stream, a, columns);
