@@ -5,7 +5,8 @@ Option names and meanings are the reference's where it has them: --model DIR, -n
 --top-p, --top-k, --min-p, --repeat-penalty, --seed, --blocks, --budget, --max-seqs,
 --no-prefix-cache, --dtype, --out, --label.  Differences: prompts are token ids (--prompt takes
 numbers separated by commas or blanks; text and tokenizers are outside this engine), and --dtype
-selects bfloat16 or float32 arithmetic rather than a quantized format.
+selects bfloat16 or float32 arithmetic rather than a quantized format; --kv-cache fp4 and --weights fp4 hold keys and
+values, and the layers' matrices, in four-bit blocks.
 """
 from __future__ import annotations
 
@@ -16,7 +17,7 @@ import time
 from typing import List
 
 USAGE = """
-  glassbox generate --model DIR --prompt IDS [-n 128] [--dtype bfloat16|float32]
+  glassbox generate --model DIR --prompt IDS [-n 128] [--dtype bfloat16|float32] [--kv-cache fp4] [--weights fp4]
                     [--temp 0] [--top-p 1] [--top-k 0] [--min-p 0] [--repeat-penalty 1] [--seed 0]
                     [--blocks 2048] [--budget 256] [--max-seqs 32] [--no-prefix-cache]
   glassbox batch    --model DIR --prompts FILE [-n 128] ...      (one prompt of ids per line; continuous batching)
@@ -44,6 +45,11 @@ def _add_model(p):
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "bf16", "float32", "f32", "fp32"])
 
 
+def _add_four_bits(p):
+    p.add_argument("--kv-cache", choices=["fp4"], help="keys and values in four-bit blocks")
+    p.add_argument("--weights", choices=["fp4"], help="the layers' matrices in four-bit blocks")
+
+
 def _add_sampling(p):
     p.add_argument("-n", type=int, default=128, dest="n")
     p.add_argument("--temp", type=float, default=0.0)
@@ -66,7 +72,7 @@ def _engine(a, blocks=None):
     from .engine import Engine
     t0 = time.time()
     eng = Engine(a.model, dtype=a.dtype, max_tokens=(blocks or a.blocks) * 16, max_seqs=getattr(a, "max_seqs", 32),
-                 prefix_caching=not getattr(a, "no_prefix_cache", True))
+                 prefix_caching=not getattr(a, "no_prefix_cache", True), kv_cache=a.kv_cache, weights=a.weights)
     print(f"loaded {eng.model.config.num_hidden_layers if hasattr(eng.model.config, 'num_hidden_layers') else len(eng.model.blocks)}"
           f" layers, {eng.model.weight_bytes() / 1e6:.0f} MB of weights in {time.time() - t0:.1f}s", file=sys.stderr)
     return eng
@@ -143,7 +149,7 @@ def cmd_bench_single(a) -> int:
     from .engine import Engine, Generator
     from .sampling import greedy_pending
     pp, tg, reps = 512, 128, 3
-    eng = Engine(a.model, dtype=a.dtype, max_tokens=pp + tg + 64, max_seqs=2)
+    eng = Engine(a.model, dtype=a.dtype, max_tokens=pp + tg + 64, max_seqs=2, kv_cache=a.kv_cache, weights=a.weights)
     vocab = eng.model.vocab_size
     prompt = [(i * 7919 + 13) % vocab for i in range(pp)]   # bench main.rs:74
     pps, tgs = [], []
@@ -164,6 +170,7 @@ def cmd_bench_single(a) -> int:
         if rep > 0:
             pps.append(p); tgs.append(d)
     res = {"engine": "glassbox_amd", "label": a.label or a.model, "model": a.model, "dtype": a.dtype,
+           "kv_cache": a.kv_cache, "weights": a.weights,
            "weight_mb": eng.model.weight_bytes() / 1e6, "pp512_tok_s": statistics.mean(pps),
            "pp512_sd": statistics.pstdev(pps), "tg128_tok_s": statistics.mean(tgs), "tg128_sd": statistics.pstdev(tgs),
            "meta": {"gpu": torch.cuda.get_device_name(0), "date": time.strftime("%Y-%m-%dT%H:%M:%SZ", time.gmtime())}}
@@ -255,7 +262,8 @@ def cmd_bench_serve(a) -> int:
         for rate in rates:
             # a cache of its own for every run, as the reference builds a scheduler for each (main.rs:245): idle
             # pages keep their prefixes, and a run must not find those of the run before
-            eng = Engine(a.model, dtype=a.dtype, max_tokens=a.blocks * 16, max_seqs=a.max_seqs, prefix_caching=prefix)
+            eng = Engine(a.model, dtype=a.dtype, max_tokens=a.blocks * 16, max_seqs=a.max_seqs, prefix_caching=prefix,
+                         kv_cache=a.kv_cache, weights=a.weights)
             vocab = eng.model.vocab_size
             prompts, outputs = serve_load(a.workload, a.requests, vocab)
             warm = [[(i * 7919 + 13 + j) % vocab for i in range(k)] for j, k in enumerate((700, 40, 300, 90))]
@@ -266,7 +274,8 @@ def cmd_bench_serve(a) -> int:
                   f"tokens reused, {r['preemptions']} preemptions", file=sys.stderr)
             runs.append({"workload": a.workload, "mode": name, "result": r})
             del eng
-    res = {"engine": "glassbox_amd", "model": a.model, "dtype": a.dtype, "token_budget": a.budget,
+    res = {"engine": "glassbox_amd", "model": a.model, "dtype": a.dtype,
+           "kv_cache": a.kv_cache, "weights": a.weights, "token_budget": a.budget,
            "max_seqs": a.max_seqs, "blocks": a.blocks, "runs": runs,
            "meta": {"gpu": torch.cuda.get_device_name(0), "date": time.strftime("%Y-%m-%dT%H:%M:%SZ", time.gmtime())}}
     text = json.dumps(res, indent=2)
@@ -354,9 +363,9 @@ def cmd_bench_kernels(a) -> int:
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="glassbox", usage=USAGE)
     sub = ap.add_subparsers(dest="cmd")
-    g = sub.add_parser("generate"); _add_model(g); _add_sampling(g); _add_serving(g)
+    g = sub.add_parser("generate"); _add_model(g); _add_four_bits(g); _add_sampling(g); _add_serving(g)
     g.add_argument("--prompt", required=True, help="token ids, separated by commas or blanks")
-    b = sub.add_parser("batch"); _add_model(b); _add_sampling(b); _add_serving(b)
+    b = sub.add_parser("batch"); _add_model(b); _add_four_bits(b); _add_sampling(b); _add_serving(b)
     b.add_argument("--prompts", required=True)
     r = sub.add_parser("random")
     r.add_argument("--config", required=True); r.add_argument("--out", required=True)
@@ -364,9 +373,9 @@ def main(argv=None) -> int:
     r.add_argument("--norm", default="ones", choices=["ones", "uniform"])
     be = sub.add_parser("bench")
     bsub = be.add_subparsers(dest="bench_cmd")
-    bs = bsub.add_parser("single"); _add_model(bs)
+    bs = bsub.add_parser("single"); _add_model(bs); _add_four_bits(bs)
     bs.add_argument("--label", default=None); bs.add_argument("--out", default=None)
-    bv = bsub.add_parser("serve"); _add_model(bv)
+    bv = bsub.add_parser("serve"); _add_model(bv); _add_four_bits(bv)
     bv.add_argument("--workload", default="chat", choices=["chat", "system", "long"])
     bv.add_argument("--requests", type=int, default=48)
     bv.add_argument("--rates", default="inf", help="requests a second, several separated by commas; inf = all at once")

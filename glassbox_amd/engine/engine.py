@@ -73,6 +73,23 @@ def sharing_obstacles(model) -> List[str]:
     return lines
 
 
+def check_four_bits(model, kv_cache: Optional[str], weights: Optional[str]) -> None:
+    """Raises EngineError, naming what is at fault, where the model cannot hold its cache or its matrices in four bits and is
+    asked to.  Needs no GPU."""
+    for name, value in (("kv_cache", kv_cache), ("weights", weights)):
+        if value not in (None, "fp4"):
+            raise EngineError(f"{name}={value!r}: None (the compute type) or 'fp4' (four bits)")
+    lines = []
+    if kv_cache == "fp4":
+        heads = ", ".join(map(str, ops.FP4_HEAD_DIMS))
+        lines += [f"kv_cache='fp4': cache layer {c}: four-bit pages are for plain attention with heads of {heads} channels"
+                  for c, spec in enumerate(model.cache_specs()) if spec is not None and not spec.four_bits]
+    if weights == "fp4":
+        lines += [f"weights='fp4': {line}" for line in model.four_bit_obstacles()]
+    if lines:
+        raise EngineError("this model cannot be held in four bits:\n  " + "\n  ".join(lines))
+
+
 class Engine:
     """model: a folder (config.json + model.safetensors) or a built and loaded model.
 
@@ -88,11 +105,16 @@ class Engine:
     is what the tuned kernels are compared with.
     layer_tapes: layers of the same parts and sizes share one walk through the parts' Python a step: the first is
     walked and its launches recorded, the others made again from native code (parts.tape); False walks every layer.
+    kv_cache: None, keys and values in the compute type; "fp4", in blocks of 32 four-bit numbers that share a power of two
+    (``ops.fp4_store``, ``ops.fp4_attention``): 4.25 bits a number, 3.76 times the tokens in the memory of a bfloat16 cache.
+    weights: None, the layers' matrices in the compute type; "fp4", in such blocks, the nearest (``ops.fp4_gemm``); the embedding
+    and the head stay as they are.  A loaded model that is handed in is quantized in place.
     """
 
     def __init__(self, model, dtype="bfloat16", max_tokens: int = 4096, max_seqs: int = 32, page_size: int = 16,
                  prefix_caching: bool = False, device: str = "cuda:0", kernels: str = "auto",
-                 graph_decode: Optional[bool] = None, layer_tapes: bool = True):
+                 graph_decode: Optional[bool] = None, layer_tapes: bool = True, kv_cache: Optional[str] = None,
+                 weights: Optional[str] = None):
         ops.require_gpu()
         self.dtype = compute_dtype(dtype)
         self.device = torch.device(device)
@@ -102,10 +124,14 @@ class Engine:
             folder = str(model)
             model = build_model(config_from_dir(folder))
             check_supported(model, self.dtype, self.page_size)      # before the weights are read
+            check_four_bits(model, kv_cache, weights)
             load_weights(model, os.path.join(folder, "model.safetensors"), self.dtype, self.device)
         else:
             check_supported(model, self.dtype, self.page_size)
-        self.model = model
+            check_four_bits(model, kv_cache, weights)
+        if weights == "fp4" and not model.quantized:
+            model.quantize()
+        self.model, self.kv_cache = model, kv_cache
         self.max_seqs = int(max_seqs)
         if kernels not in ("auto", "plain"):
             raise EngineError(f"kernels={kernels!r}: 'auto' (tuned and fused kernels where they apply) or 'plain'")
@@ -138,9 +164,14 @@ class Engine:
                 lc.group = keys.index(spec.group_key)
                 # one page and one state slot more than the manager hands out: filler rows of a replayed step
                 # write there (engine.decode_graphs)
-                shape = ops.key_pages_shape(num_pages + 1, spec.num_kv_heads, self.page_size, spec.head_dim)
-                lc.k_pages = torch.zeros(shape, dtype=self.dtype, device=self.device)
-                if spec.values:
+                if kv_cache == "fp4":
+                    shape = ops.fp4_pages_shape(num_pages + 1, spec.num_kv_heads, self.page_size, spec.head_dim)
+                    lc.k_pages = torch.zeros(shape, dtype=torch.uint8, device=self.device)
+                    lc.v_pages = torch.zeros_like(lc.k_pages)
+                else:
+                    shape = ops.key_pages_shape(num_pages + 1, spec.num_kv_heads, self.page_size, spec.head_dim)
+                    lc.k_pages = torch.zeros(shape, dtype=self.dtype, device=self.device)
+                if spec.values and lc.v_pages is None:
                     lc.v_pages = torch.zeros((num_pages + 1, spec.num_kv_heads, spec.head_dim, self.page_size),
                                              dtype=self.dtype, device=self.device)   # transposed: see ops._check_pages
             if state is not None:

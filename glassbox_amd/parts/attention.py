@@ -16,7 +16,7 @@ import torch
 
 from .. import ops
 from .base import (FULL, RUNS, WINDOW, CacheSpec, LayerCache, Mixer, PositionEncoding, PreNormed, StateSpec, TensorSpec, emit_target,
-                   needs_multiple_of_8, product, product_in_slices, split_workspace)
+                   fp4_product, needs_multiple_of_8, needs_multiple_of_32, product, product_in_slices, split_workspace)
 
 
 def paged_attention(ctx, q: torch.Tensor, out: torch.Tensor, cache: LayerCache, n_heads: int, scale: float,
@@ -63,6 +63,18 @@ def paged_attention(ctx, q: torch.Tensor, out: torch.Tensor, cache: LayerCache, 
         ops.attention_prefill(q, out, ctx, cache, n_heads, scale, window, keep_first, chunk, softcap, sinks, slopes=slopes)
 
 
+def fp4_paged_attention(ctx, q: torch.Tensor, out: torch.Tensor, cache: LayerCache, n_heads: int, scale: float, window: int) -> None:
+    """Attention of every row of the step over its request's four-bit pages: the requests with one row, then the portions."""
+    _, n_kv, blocks, _, _ = cache.k_pages.shape
+    tables, n_decode, longest = ctx.tables[cache.group], ctx.host["n_decode"], int(ctx.host["max_context"])
+    for a, b, rows in ((0, n_decode, 1), (n_decode, ctx.num_seqs, int(ctx.host["max_q_len"]))):
+        if a < b:
+            floats = ops.fp4_attention_floats(b - a, n_heads, n_kv, blocks * ops.FP4_BLOCK, rows, longest, window, ctx.dtype)
+            ops.fp4_attention(q, out, ctx.q_start[a:b], ctx.q_len[a:b], ctx.pos0[a:b], tables[a:b], cache.k_pages, cache.v_pages, n_heads,
+                              scale, rows, longest, window=window,
+                              workspace=ctx.buffer("fp4_attention", (floats,), torch.float32) if floats else None)
+
+
 class PagedAttention(Mixer):
     replayable = True
     taped = True
@@ -78,10 +90,12 @@ class PagedAttention(Mixer):
         self.scale = float(scale) if scale is not None else 1.0 / math.sqrt(head_dim)  # model.rs:244
         self.q_dim = n_heads * head_dim
         self.kv_dim = n_kv_heads * head_dim
-        self.cache_spec = None if shares_kv else CacheSpec(n_kv_heads, head_dim,
-                                                           WINDOW if window > 0 else FULL, self.window)
-        self.wqkv: Optional[torch.Tensor] = None
+        self.cache_spec = None if shares_kv else CacheSpec(n_kv_heads, head_dim, WINDOW if window > 0 else FULL, self.window,
+                                                           four_bits=head_dim in ops.FP4_HEAD_DIMS)
+        self.wqkv: Optional[torch.Tensor] = None          # (four-bit codes, with the scales below, after ``quantize``)
         self.wo: Optional[torch.Tensor] = None
+        self.wqkv_scales: Optional[torch.Tensor] = None
+        self.wo_scales: Optional[torch.Tensor] = None
 
     def tensor_specs(self) -> Dict[str, TensorSpec]:
         specs = {"q_proj.weight": TensorSpec((self.q_dim, self.width))}
@@ -107,9 +121,18 @@ class PagedAttention(Mixer):
             # one product computes all three (model.rs:59-61)
             self.wqkv = torch.cat([tensors["q_proj.weight"], tensors["k_proj.weight"], tensors["v_proj.weight"]], 0)
         self.wo = tensors["o_proj.weight"].contiguous()
+        self.wqkv_scales = self.wo_scales = None
 
     def streamed_matrices(self):
-        return [self.wqkv, self.wo]
+        return [t for t in (self.wqkv, self.wo, self.wqkv_scales, self.wo_scales) if t is not None]
+
+    def four_bit_obstacles(self):
+        return needs_multiple_of_32("width", self.width) + needs_multiple_of_32("n_heads * head_dim", self.q_dim)
+
+    def quantize(self):
+        if self.wqkv_scales is None:
+            self.wqkv, self.wqkv_scales = ops.fp4_quantize(self.wqkv)
+            self.wo, self.wo_scales = ops.fp4_quantize(self.wo)
 
     def problems(self, dtype, page_size):
         out = needs_multiple_of_8(dtype, "width", self.width) + needs_multiple_of_8(dtype, "n_heads * head_dim", self.q_dim)
@@ -126,6 +149,8 @@ class PagedAttention(Mixer):
         projection may prepare the norm that reads the residual next (returns a PreNormed if it did)."""
         if cache is None or cache.k_pages is None:
             raise ValueError("PagedAttention needs a layer cache with pages")
+        if self.wqkv_scales is not None or cache.k_pages.dtype == torch.uint8:
+            return self._forward_fp4(ctx, h, residual, cache, norm, emit)
         n = h.shape[0]
         rows = self.q_dim + (0 if self.shares_kv else 2 * self.kv_dim)
         qkv = ctx.buffer("qkv", (n, rows), ctx.dtype)
@@ -168,6 +193,44 @@ class PagedAttention(Mixer):
         target, handed_on = emit_target(ctx, n, self.width, self.q_dim, emit, "mixer")
         ops.gemm(att, self.wo, residual, accumulate=True, emit=target,
                  workspace=split_workspace(ctx, n, self.width, self.q_dim))
+        return handed_on
+
+    def _forward_fp4(self, ctx, h, residual, cache: LayerCache, norm, emit):
+        """``forward`` with matrices or pages, or both, of four-bit numbers: the norm (where the product does not take it), the
+        product, rotation and cache write, attention and the output projection are a launch each."""
+        n = h.shape[0]
+        rows = self.q_dim + (0 if self.shares_kv else 2 * self.kv_dim)
+        n_kv = 0 if self.shares_kv else self.n_kv_heads
+        qkv = ctx.buffer("qkv", (n, rows), ctx.dtype)
+        packed, pre = self.wqkv_scales is not None, isinstance(norm, PreNormed)
+        if norm is not None and not pre and (packed or ctx.dtype == torch.float32):
+            normed = ctx.buffer("h", (n, self.width), ctx.dtype)
+            ops.rmsnorm(h, norm[0], norm[1], normed)
+            h, norm = normed, None
+        if packed:   # (never with ``pre``: the matrices before this one are packed too, and their products prepare no norm)
+            fp4_product(ctx, h, self.wqkv, self.wqkv_scales, qkv)
+        elif pre:
+            ops.gemm(norm.rows, self.wqkv, qkv, rms_parts=norm.as_gemm_arg())
+        else:
+            ops.gemm(h, self.wqkv, qkv, rms=norm, workspace=None if norm is not None else split_workspace(ctx, n, rows, self.width))
+        slots = ctx.slots[cache.group] if cache.writable and not self.shares_kv else None
+        att = ctx.buffer("att", (n, self.q_dim), ctx.dtype)
+        if cache.k_pages.dtype == torch.uint8:
+            angles = self.position.fuse_spec(ctx, self.head_dim)
+            if angles is None:   # an encoding that does its own work does it in place; the heads are then stored as they are
+                self.position.apply_and_store(ctx, qkv, self.n_heads, n_kv, self.head_dim, None, None, None)
+                angles = (None, None)
+            ops.fp4_store(qkv, *angles, slots, cache.k_pages, cache.v_pages, self.n_heads, n_kv, self.head_dim)
+            fp4_paged_attention(ctx, qkv[:, :self.q_dim], att, cache, self.n_heads, self.scale, self.window)
+        else:
+            store = (slots, cache.k_pages, cache.v_pages) if slots is not None else (None, None, None)
+            self.position.apply_and_store(ctx, qkv, self.n_heads, n_kv, self.head_dim, *store)
+            paged_attention(ctx, qkv[:, :self.q_dim], att, cache, self.n_heads, self.scale, self.window)
+        if packed:
+            fp4_product(ctx, att, self.wo, self.wo_scales, residual, accumulate=True)
+            return None
+        target, handed_on = emit_target(ctx, n, self.width, self.q_dim, emit, "mixer")
+        ops.gemm(att, self.wo, residual, accumulate=True, emit=target, workspace=split_workspace(ctx, n, self.width, self.q_dim))
         return handed_on
 
 

@@ -60,13 +60,15 @@ class CacheSpec:
     """Paged keys and values of one layer.  kind FULL keeps every position, WINDOW the last ``window`` and, with
     ``keep_first``, the first so many as well; RUNS the positions of the run of ``window`` (runs counted from the
     request's first position) that holds the next query.  ``values`` False: pages of keys alone, for a mixer that caches one
-    row a position and makes everything else of it."""
+    row a position and makes everything else of it.  ``four_bits``: the mixer also takes pages of four-bit numbers
+    (``ops.fp4_pages_shape``; the engine's ``kv_cache``)."""
     num_kv_heads: int
     head_dim: int
     kind: int = FULL
     window: int = 0
     keep_first: int = 0
     values: bool = True
+    four_bits: bool = False
 
     @property
     def group_key(self) -> Tuple[int, int, int]:
@@ -88,6 +90,7 @@ class LayerCache:
     """What the engine hands a mixer: its layer's pages, the index of their page group, its state."""
     k_pages: Optional[torch.Tensor] = None   # [pages, kv heads, head size / piece, page size, piece] (ops.key_pages_shape)
     v_pages: Optional[torch.Tensor] = None   # [pages, kv heads, head size, page size] (transposed); None: keys alone
+    # (both uint8: pages of four-bit numbers, ops.fp4_pages_shape)
     group: int = 0
     state: Optional[torch.Tensor] = None     # [slots, *state shape]
     state_initial: float = 0.0               # what a slot holds when its request starts
@@ -157,6 +160,31 @@ class Part:
         for child in self.children().values():
             out.extend(child.problems(dtype, page_size))
         return out
+
+    def four_bit_obstacles(self) -> List[str]:
+        """Why the matrices of this part cannot be held in four bits, a line for each reason (empty if they can, or if there
+        are none).  By default a part with matrices of its own has no products for such, and the children are asked."""
+        own = [f"{type(self).__name__} has no products with four-bit matrices"] if any(
+            s.kind == "matrix" and len(s.shape) > 1 for s in self.tensor_specs().values()) else []
+        return own + [line for child in self.children().values() for line in child.four_bit_obstacles()]
+
+    def quantize(self) -> None:
+        """Holds the loaded matrices of this part in four bits from now on; called where ``four_bit_obstacles`` is empty."""
+        for child in self.children().values():
+            child.quantize()
+
+
+def needs_multiple_of_32(what: str, size: int) -> List[str]:
+    """Four-bit matrices are blocks of 32 numbers of their inner size."""
+    return [f"{what}: {size} is not a multiple of 32, the block of a four-bit matrix"] if size % 32 else []
+
+
+def fp4_product(ctx, a, codes, scales, out, accumulate: bool = False, silu_mul: bool = False) -> None:
+    """``ops.fp4_gemm`` with the workspace that it has a use for in this step."""
+    from .. import ops
+    floats = ops.fp4_gemm_floats(a.shape[0], codes.shape[0], a.shape[1], a.dtype, out.dtype, silu_mul)
+    ops.fp4_gemm(a, ops.Fp4Matrix(codes, scales), out, accumulate=accumulate, silu_mul=silu_mul,
+                 workspace=ctx.buffer("fp4_gemm", (floats,), torch.float32) if floats else None)
 
 
 def needs_multiple_of_8(dtype: torch.dtype, what: str, size: int) -> List[Tuple[str, str]]:

@@ -7,8 +7,8 @@ from typing import Dict, Optional
 import torch
 
 from .. import ops
-from .base import (FeedForward, PreNormed, TensorSpec, emit_target, needs_multiple_of_8, product, product_in_slices,
-                   split_workspace)
+from .base import (FeedForward, PreNormed, TensorSpec, emit_target, fp4_product, needs_multiple_of_8, needs_multiple_of_32, product,
+                   product_in_slices, split_workspace)
 
 
 class SwiGLU(FeedForward):
@@ -19,8 +19,10 @@ class SwiGLU(FeedForward):
         """``any_size``: sizes that the bfloat16 matrix-core products do not take (no multiples of 8) are not refused but
         go through the plain product, unfused."""
         self.width, self.intermediate, self.any_size = width, intermediate, bool(any_size)
-        self.w_gate_up: Optional[torch.Tensor] = None
+        self.w_gate_up: Optional[torch.Tensor] = None     # (four-bit codes, with the scales below, after ``quantize``)
         self.w_down: Optional[torch.Tensor] = None
+        self.w_gate_up_scales: Optional[torch.Tensor] = None
+        self.w_down_scales: Optional[torch.Tensor] = None
 
     def tensor_specs(self) -> Dict[str, TensorSpec]:
         return {"gate_proj.weight": TensorSpec((self.intermediate, self.width)),
@@ -30,9 +32,18 @@ class SwiGLU(FeedForward):
     def load(self, tensors):
         self.w_gate_up = torch.cat([tensors["gate_proj.weight"], tensors["up_proj.weight"]], 0)
         self.w_down = tensors["down_proj.weight"].contiguous()
+        self.w_gate_up_scales = self.w_down_scales = None
 
     def streamed_matrices(self):
-        return [self.w_gate_up, self.w_down]
+        return [t for t in (self.w_gate_up, self.w_down, self.w_gate_up_scales, self.w_down_scales) if t is not None]
+
+    def four_bit_obstacles(self):
+        return needs_multiple_of_32("width", self.width) + needs_multiple_of_32("intermediate", self.intermediate)
+
+    def quantize(self):
+        if self.w_gate_up_scales is None:
+            self.w_gate_up, self.w_gate_up_scales = ops.fp4_quantize(self.w_gate_up)
+            self.w_down, self.w_down_scales = ops.fp4_quantize(self.w_down)
 
     def problems(self, dtype, page_size):
         if self.any_size:
@@ -50,6 +61,14 @@ class SwiGLU(FeedForward):
         ``store``: the rows are written to ``residual`` (float32) instead of added."""
         n = h.shape[0]
         act = ctx.buffer("act", (n, self.intermediate), ctx.dtype)
+        if self.w_gate_up_scales is not None:   # (no PreNormed: the mixer's matrices are packed too, and their products prepare no norm)
+            if norm is not None:
+                normed = ctx.buffer("h", (n, self.width), ctx.dtype)
+                ops.rmsnorm(h, norm[0], norm[1], normed)
+                h = normed
+            fp4_product(ctx, h, self.w_gate_up, self.w_gate_up_scales, act, silu_mul=True)
+            fp4_product(ctx, act, self.w_down, self.w_down_scales, residual, accumulate=not store)
+            return None
         if ctx.dtype == torch.bfloat16 and (self.width % 8 or self.intermediate % 8):
             # (only with ``any_size``, and then without norms to fuse: the blocks that offer those build it without)
             gate_up = ctx.buffer("gate_up", (n, 2 * self.intermediate), ctx.dtype)

@@ -89,6 +89,7 @@ class DecoderModel(Part):
         self._check_schedule()
         self._taped: Optional[List[bool]] = None       # which blocks let their launches be recorded (parts.tape)
         self.loads = 0                                # times the weights were loaded: recorded tensors are theirs
+        self.quantized = False                        # the layers' matrices are held in four bits (``quantize``)
 
     # structure ------------------------------------------------------------------
     def children(self) -> Dict[str, Part]:
@@ -246,6 +247,23 @@ class DecoderModel(Part):
     def load_tree(self, tensors, prefix: str = "") -> None:
         super().load_tree(tensors, prefix)
         self.loads += 1   # what engines keep of the layers' tensors (parts.tape) is of the weights before
+        if self.quantized:
+            self.quantize()
+
+    def four_bit_obstacles(self) -> List[str]:
+        """Those of the layers; a line that many layers share is given once, with the first that has it."""
+        first: Dict[str, str] = {}
+        for i, block in enumerate(self.blocks):
+            for line in block.four_bit_obstacles():
+                first.setdefault(line, self.names[1].format(i))
+        return [f"{name}: {line}" for line, name in first.items()]
+
+    def quantize(self) -> None:
+        """Holds the layers' matrices in four bits, these and any loaded later.  The embedding and the head stay as they are."""
+        for block in self.blocks:
+            block.quantize()
+        self.quantized = True
+        self.loads += 1
 
     def streamed_matrices(self) -> List[torch.Tensor]:
         """Every tensor a step reads whole, once each: those of the scheduled blocks (a block named twice, or a

@@ -4,6 +4,11 @@ import math
 import pytest
 import torch
 
+import dekinex_cases
+import helpers
+import sagalorn_cases
+import tekilix_cases
+import zakusun_cases
 from glassbox_amd import ops
 
 BF, F32, I32, U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
@@ -85,3 +90,31 @@ def test_sizes():
     assert ops.fp4_pages_shape(7, 3, 32, 128) == (7, 3, 4, 17, 32)
     assert [ops.fp4_scale_bytes(k) for k in (32, 512, 544, 4096)] == [16, 16, 32, 128]
     assert ops.Fp4Matrix(torch.zeros(10, 32, dtype=U8), torch.zeros(10, 16, dtype=U8)).shape == (10, 64)
+
+
+def model_of(config):
+    from glassbox_amd.config import config_from_dict
+    from glassbox_amd.weights import build_model
+    return build_model(config_from_dict(config))
+
+
+@pytest.mark.parametrize("config,kv_cache,weights,why", [
+    (helpers.TINY_E, "fp4", None, "cache layer 0: four-bit pages are for plain attention with heads of 32"),     # heads of 16
+    (helpers.TINY_E, None, "fp4", "width: 72 is not a multiple of 32"), (helpers.TINY_E, None, "fp4", "intermediate: 120 is not a multiple"),
+    (helpers.TINY_A, None, "fp4", "intermediate: 176"), (helpers.TINY_B, "fp8", None, "kv_cache='fp8'"), (helpers.TINY_B, None, "int4", "weights='int4'"),
+    (zakusun_cases.CASES["A"], "fp4", None, "four-bit pages"), (zakusun_cases.CASES["A"], None, "fp4", "has no products with four-bit"),
+    (tekilix_cases.CASES["A"], "fp4", None, "four-bit pages"), (tekilix_cases.CASES["A"], None, "fp4", "has no products with four-bit"),
+    (dekinex_cases.CASES["A"], None, "fp4", "has no products with four-bit"), (sagalorn_cases.CASES["P"], None, "fp4", "has no products with four-bit"),
+])
+def test_models_that_cannot(config, kv_cache, weights, why):
+    from glassbox_amd.engine.engine import EngineError, check_four_bits
+    model = model_of(config)
+    with pytest.raises(EngineError, match=why):
+        check_four_bits(model, kv_cache, weights)
+    check_four_bits(model, None, None)
+
+
+@pytest.mark.parametrize("config", [helpers.TINY_B, helpers.WIDE_W, helpers.MID_M])
+def test_models_that_can(config):
+    from glassbox_amd.engine.engine import check_four_bits
+    check_four_bits(model_of(config), "fp4", "fp4")
