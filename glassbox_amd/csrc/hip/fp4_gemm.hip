@@ -16,6 +16,7 @@
 #include "fp4.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace gb {
 
@@ -84,7 +85,9 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(MT * 
   constexpr int SP = kFp4Terms<T>;
   const int lane = threadIdx.x % kWave, r = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int nt = blockIdx.x;
+  // the row tiles of one tile of W follow each other on one XCD (workgroups go to the eight in turn), whose L2 then has it
+  const int order = blockIdx.x / 8, nt = order / a.m_tiles * 8 + blockIdx.x % 8, mt0 = order % a.m_tiles * 8 * MT;
+  if (nt >= a.n_tiles) return;
   const bool silu = a.epilogue == 2;
   const int half = a.N / 2;
   const uint8_t *codes[NT], *scales[NT];
@@ -97,7 +100,7 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(MT * 
     scales[p] = a.scales + (size_t)row * a.scale_stride;
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) x[t] = (const T*)a.x + (size_t)min(t * 8 + r % 8, a.M - 1) * a.ldx;
+  for (int t = 0; t < MT; ++t) x[t] = (const T*)a.x + (size_t)min(mt0 + t * 8 + r % 8, a.M - 1) * a.ldx;
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int p = 0; p < NT; ++p)
@@ -183,7 +186,7 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(MT * 
   };
   if (silu && !a.slices) {
     for (int u = wave; u < NT / 2 * MT; u += W) {
-      const int p = u / MT * 2, t = u % MT, m = 8 * t + r;
+      const int p = u / MT * 2, t = u % MT, m = mt0 + 8 * t + r;
       const f32x4 gate = total(p * MT + t), up = total((p + 1) * MT + t);
       f32x4 v;
 #pragma unroll
@@ -192,7 +195,7 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(MT * 
     }
   } else {
     for (int u = wave; u < NT * MT; u += W) {
-      const int p = u / MT, t = u % MT, m = 8 * t + r;
+      const int p = u / MT, t = u % MT, m = mt0 + 8 * t + r;
       const f32x4 v = total(u);
       if (m < a.M && r < 8 && g < 2) put_or_leave(a, m, row_of(p) + 4 * g, silu && !(p & 1) ? half : a.N, v);
     }
@@ -207,8 +210,7 @@ __global__ __launch_bounds__(256) void fp4_tiles_kernel(GemmArgs a) {
   __shared__ bf16x8 xs[2][SP][kRows * kWords];
   const int lane = threadIdx.x % kWave, r = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  // the row tiles of one tile of W follow each other on one XCD (workgroups go to the eight in turn), whose L2 then has it
-  const int order = blockIdx.x / 8, nt = order / a.m_tiles * 8 + blockIdx.x % 8, mt0 = order % a.m_tiles * kRows;
+  const int order = blockIdx.x / 8, nt = order / a.m_tiles * 8 + blockIdx.x % 8, mt0 = order % a.m_tiles * kRows;   // (as above)
   if (nt >= a.n_tiles) return;
   const bool silu = a.epilogue == 2;
   const int half = a.N / 2;
@@ -347,43 +349,68 @@ __global__ __launch_bounds__(256) void fp4_gemm_join_kernel(GemmArgs a, int slic
 
 // Which kernel takes a product, and how: a function of its sizes and type alone.
 struct Form {
-  int rows_w, rows_a, step;   // a workgroup's rows of W and of a, blocks of k a turn
+  int rows_w, rows_a, step;          // a workgroup's rows of W and of a, blocks of k a turn
+  float alone[2], busy[2];           // us of a turn with little and with much on the chip (bf16 rows, 32-bit ones), 0: not for such rows
 };
-// lines: MT x NT, waves (a turn is 8 U blocks a wave)      1 x 4, 8       1 x 2, 8       1 x 1, 8 (U 2)   2 x 8, 4        2 x 4, 8
-// tiles: MT x NT, blocks                                   2 x 2, 8       4 x 2, 8       4 x 4, 4         2 x 2, 4 and 4 x 2, 4 (32-bit rows)
-static constexpr Form kForms[] = {{32, 8, 64}, {16, 8, 64}, {8, 8, 128}, {64, 16, 32}, {32, 16, 64}, {128, 32, 8}, {128, 64, 8}, {256, 64, 4},
-                                  {128, 32, 4}, {128, 64, 4}};
+static constexpr int kLinesForms = 5;
+static constexpr Form kForms[] = {{32, 8, 64, {0.f, 0.f}, {1.9f, 3.1f}},         // lines: MT x NT 1 x 4, 8 waves
+                                  {16, 8, 64, {0.f, 0.f}, {1.35f, 2.3f}},        // 1 x 2, 8
+                                  {8, 8, 128, {0.f, 0.f}, {1.7f, 3.7f}},         // 1 x 1, 8 (U 2)
+                                  {64, 16, 32, {0.f, 0.f}, {2.3f, 4.9f}},        // 2 x 8, 4
+                                  {32, 16, 64, {0.f, 0.f}, {2.9f, 5.5f}},        // 2 x 4, 8
+                                  {64, 32, 8, {0.95f, 0.f}, {0.6f, 0.f}},        // tiles: 2 x 1, 8 blocks
+                                  {128, 32, 8, {1.4f, 0.f}, {1.05f, 0.f}},       // 2 x 2, 8
+                                  {128, 64, 8, {2.f, 0.f}, {1.4f, 0.f}},         // 4 x 2, 8
+                                  {256, 64, 4, {1.65f, 0.f}, {1.05f, 0.f}},      // 4 x 4, 4
+                                  {64, 32, 4, {0.f, 1.2f}, {0.f, 0.67f}},        // 2 x 1, 4
+                                  {128, 32, 4, {0.f, 1.35f}, {0.f, 0.87f}}};     // 2 x 2, 4
 struct Plan {
   int form, n_tiles, m_tiles, turns, slices;
 };
 
-static Plan plan(int M, int N, int K, bool silu, int dtype) {
-  auto tiles = [&](int form) { return (long long)((N + kForms[form].rows_w - 1) / kForms[form].rows_w) * ((M + kForms[form].rows_a - 1) / kForms[form].rows_a); };
-  Plan p;
+static Plan plan(int M, int N, int K, bool silu, int dtype, int most_slices) {
+  auto laid_out = [&](int form, int slices) {
+    const Form& f = kForms[form];
+    Plan p{form, silu ? (N / 2 + f.rows_w / 2 - 1) / (f.rows_w / 2) : (N + f.rows_w - 1) / f.rows_w, (M + f.rows_a - 1) / f.rows_a, 0, 0};
+    const int turns = (K / 32 + f.step - 1) / f.step;
+    p.turns = (turns + slices - 1) / slices;
+    p.slices = (turns + p.turns - 1) / p.turns;
+    return p;
+  };
   // up to 8 rows: as many rows of W a workgroup as leave about 192 of them (16 with silu, which takes pairs of tiles).  us, 8 rows: 6,144 of
-  // 4,096 by 32 7.8, by 16 8.5; 4,096 of 14,336 by 16 14.1, by 32 21; 2,048 of 8,192 by 8 8.1, by 16 11.
-  if (M <= 8) p.form = N >= 6144 ? 0 : N >= 4096 || silu ? 1 : 2;
-  // up to 16: 28,672 of 4,096 by 64 24.2, by 32 29; 6,144 of 4,096 by 32 9.8, by 64 14
-  else if (M <= 16) p.form = N >= 16384 ? 3 : 4;
-  // more: 64 x 256 where there are enough of them: 256 rows by 28,672 of 4,096 82 (64 x 128 87), by 4,096 of 4,096 27 (24.5)
-  else if (dtype == kF32) p.form = M <= 32 ? 8 : 9;
-  else p.form = M <= 32 ? 5 : tiles(7) >= 384 ? 7 : 6;
-  const Form f = kForms[p.form];
-  p.n_tiles = silu ? (N / 2 + f.rows_w / 2 - 1) / (f.rows_w / 2) : (N + f.rows_w - 1) / f.rows_w;
-  p.m_tiles = (M + f.rows_a - 1) / f.rows_a;
-  const int turns = (K / 32 + f.step - 1) / f.step;
-  // slices of k, us: 16 rows by 4,096 of 14,336 in 2 18.3 (1: 29); 32 in 8 19.9 (1: 41); 128 in 8 33.1; 64 by 4,096 of 4,096 in 8 15.9 (1: 21)
-  const long long groups = (long long)p.n_tiles * p.m_tiles;
-  const long long want = M <= 8 ? 1 : M <= 16 ? 256 / groups : groups <= 224 ? (384 + groups - 1) / groups : 1;
-  const int slices = (int)std::max<long long>(1, std::min<long long>(want, turns));
-  p.turns = (turns + slices - 1) / slices;
-  p.slices = (turns + p.turns - 1) / p.turns;
-  return p;
+  // 4,096 by 32 7.8, by 16 8.5; 2,560 of 2,560 by 16 5.3, by 8 6.1; 2,048 of 8,192 by 8 8.1, by 16 11.
+  if (M <= 8) return laid_out(N >= 6144 ? 0 : N >= 2560 || silu ? 1 : 2, 1);
+  // more: the form with the least time by a model, whose numbers are fitted to 21 products of 9 to 1,024 rows in every form, with weights from
+  // memory (8 % off; its choice is 1 to 2 % slower than the best).  A product costs its launch, W's bytes at 11 TB/s, and its turns, one after
+  // another, each as long as its own latency or as what the workgroups of a compute unit need together (lines: the blocks that the waves
+  // take, and some); slices a second launch and the way of the sums out and back.  us, best and next:
+  // 16 rows by 28,672 of 4,096 64 x 16 24, 128 x 32 in two 27; 64 by 6,144 of 2,048 64 x 32 9.7, 128 x 64 in eight 16; by 4,096 of 14,336 128 x 64
+  // in eight 24, 64 x 32 in four 25; 256 by 28,672 of 4,096 256 x 64 81, 128 x 64 94; 32-bit rows, 32 by 2,048 of 2,048 64 x 32 in eight 8.1, 128 x 32 8.8
+  const int t = dtype == kF32;
+  float least = 0.f;
+  Plan best{-1, 0, 0, 0, 0};
+  for (int form = 0; form < (int)(sizeof kForms / sizeof *kForms); ++form) {
+    const Form& f = kForms[form];
+    if (f.busy[t] == 0.f || (silu && f.rows_w < 128 && (form >= kLinesForms || f.rows_w == 8))) continue;   // (silu: pairs of tiles a wave)
+    for (int slices : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      const Plan p = laid_out(form, slices);
+      const float groups = (float)p.n_tiles * p.m_tiles;
+      if (p.slices != slices || slices > most_slices || (slices > 1 && groups * (slices - 1) > 512)) continue;
+      const float each = groups * slices / 256, shared = each > 8 ? each + 0.5f : std::ceil(each);   // workgroups a compute unit
+      const bool lines = form < kLinesForms;
+      float us = (lines ? 3.1f : 2.1f) + (float)N * K * 4.8e-8f;
+      if (lines) us += (std::min((float)p.turns, K / 32.f / f.step / slices) + 0.2f) * f.busy[t] * shared;
+      else us += p.turns * std::max(f.alone[t], f.busy[t] * shared);
+      if (slices > 1) us += 2.7f + slices * (float)M * N / 440e3f;
+      if (best.form < 0 || us < least) least = us, best = p;
+    }
+  }
+  return best;
 }
 
 template <typename T, int MT, int NT, int W, int U> static void lines(const Plan& p, const GemmArgs& a, hipStream_t stream) {
   static_assert(MT * NT * W <= 64, "the waves' sums fill LDS");
-  hipLaunchKernelGGL((fp4_lines_kernel<T, MT, NT, W, U>), dim3((unsigned)p.n_tiles, (unsigned)p.slices), dim3(W * kWave), 0, stream, a);
+  hipLaunchKernelGGL((fp4_lines_kernel<T, MT, NT, W, U>), dim3((unsigned)((p.n_tiles + 7) / 8 * 8 * p.m_tiles), (unsigned)p.slices), dim3(W * kWave), 0, stream, a);
 }
 template <typename T, int MT, int NT, int B> static void tiles(const Plan& p, const GemmArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((fp4_tiles_kernel<T, MT, NT, B>), dim3((unsigned)((p.n_tiles + 7) / 8 * 8 * p.m_tiles), (unsigned)p.slices), dim3(256), 0, stream, a);
@@ -398,11 +425,12 @@ template <typename T> static void launch_by(const Plan& p, const GemmArgs& a, hi
     case 4: lines<T, 2, 4, 8, 1>(p, a, stream); break;
     default:
       if constexpr (std::is_same_v<T, float>) {
-        if (p.form == 8) tiles<T, 2, 2, 4>(p, a, stream);
-        else tiles<T, 4, 2, 4>(p, a, stream);
+        if (p.form == 9) tiles<T, 2, 1, 4>(p, a, stream);
+        else tiles<T, 2, 2, 4>(p, a, stream);
       } else {
-        if (p.form == 5) tiles<T, 2, 2, 8>(p, a, stream);
-        else if (p.form == 6) tiles<T, 4, 2, 8>(p, a, stream);
+        if (p.form == 5) tiles<T, 2, 1, 8>(p, a, stream);
+        else if (p.form == 6) tiles<T, 2, 2, 8>(p, a, stream);
+        else if (p.form == 7) tiles<T, 4, 2, 8>(p, a, stream);
         else tiles<T, 4, 4, 4>(p, a, stream);
       }
   }
@@ -419,7 +447,7 @@ using namespace gb;
 // floats of workspace with which k is divided; 0: it is not
 extern "C" long long gb_fp4_gemm_floats(int M, int N, int K, int epilogue, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const Plan p = plan(M, N, K, epilogue == 2, dtype);
+  const Plan p = plan(M, N, K, epilogue == 2, dtype, 16);
   return p.slices > 1 ? (long long)p.slices * M * N : 0;
 }
 
@@ -433,11 +461,8 @@ extern "C" int gb_fp4_gemm(const void* x, int dtype, int ldx, const void* codes,
              "fp4_gemm: codes and scales begin at 16-byte words, rows of scales are multiples of 16");
   GB_REQUIRE((dtype == kF32 || dtype == kBF16) && (out_dtype == kF32 || out_dtype == kBF16), "fp4_gemm: unknown dtype %d or %d", dtype, out_dtype);
   if (M == 0) return 0;
-  Plan p = plan(M, N, K, epilogue == 2, dtype);
-  if (p.slices > 1 && (!workspace || workspace_floats < (long long)p.slices * M * N)) {   // whole k a workgroup: slower, not refused
-    p.turns *= p.slices;
-    p.slices = 1;
-  }
+  Plan p = plan(M, N, K, epilogue == 2, dtype, 16);
+  if (p.slices > 1 && (!workspace || workspace_floats < (long long)p.slices * M * N)) p = plan(M, N, K, epilogue == 2, dtype, 1);   // slower, not refused
   GB_REQUIRE((long long)(p.n_tiles + 7) * p.m_tiles < (1ll << 31) && (long long)M * N < (1ll << 38), "fp4_gemm: %d x %d is too much for one launch", M, N);
   const int e = out_dtype == kF32 ? 16 : 8;   // bytes of four columns
   const GemmArgs a{x, (const uint8_t*)codes, (const uint8_t*)scales, out, p.slices > 1 ? workspace : nullptr, ldx, ldo, M, N, K / 32, scale_stride,

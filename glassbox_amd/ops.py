@@ -2792,9 +2792,11 @@ def fp4_expand(w: Fp4Matrix, out: torch.Tensor) -> None:
 
 def _fp4_expands(rows: int, n: int, k: int, dtype: torch.dtype, out_dtype: torch.dtype, silu_mul: bool) -> bool:
     """Whether a product goes through the weights' bfloat16 values, given the workspace for them: ``gemm`` takes many rows in fewer us than the
-    kernel that converts on the way, and more than the values cost: 2,048 rows by 28,672 of 4,096 59 + 417 us and 534, by 4,096 of 4,096 8.5
-    + 75.5 and 80."""
-    return (rows >= 1536 and n * k >= 1 << 26 and dtype == torch.bfloat16 and not (silu_mul and (n % 16 or out_dtype != torch.bfloat16)))
+    kernel that converts on the way, and more than the values cost: 2,048 rows by 28,672 of 4,096 428 and 537, by 6,144 of 2,048 51 and 69;
+    768 by 4,096 of 14,336 115 and 153.  Not so for fewer rows (512 by 4,096 of 14,336 93 and 87) or numbers (2,048 by 1,600 of 960 20 and 15)."""
+    size = n * k
+    return (dtype == torch.bfloat16 and (rows >= 1536 and size >= 1 << 22 or rows >= 768 and size >= 1 << 24)
+            and not (silu_mul and (n % 16 or out_dtype != torch.bfloat16)))
 
 
 @functools.lru_cache(maxsize=4096)   # a pure function of the sizes, asked for at every product

@@ -330,7 +330,10 @@ def test_attention_and_store_reach_pages_beyond_four_gigabytes():
 
 # ------------------------------------------------------------------------------------------------------------------- products
 GEMMS = [(1, 1, 32), (1, 40, 64), (3, 17, 96), (16, 64, 512), (17, 130, 544), (5, 2563, 992), (33, 300, 2048), (64, 96, 4128), (65, 48, 160),
-         (130, 1040, 256), (16, 17000, 96), (9, 520, 4128), (1, 8200, 1056), (2, 33000, 128), (20, 16500, 160), (300, 70, 992)]
+         (130, 1040, 256), (16, 17000, 96), (9, 520, 4128), (1, 8200, 1056), (2, 33000, 128), (20, 16500, 160), (300, 70, 992),
+         # (each of the kernels' forms, with k whole and divided, one tile of rows and several)
+         (9, 4100, 544), (9, 8200, 544), (17, 4100, 544), (9, 2050, 8224), (30, 1040, 8224), (17, 520, 8224), (9, 4100, 4128), (700, 70, 4128),
+         (33, 6150, 2080), (65, 12300, 96), (65, 6150, 4128), (33, 6150, 8224), (130, 1000, 960)]
 
 
 @pytest.mark.parametrize("M,N,K", GEMMS)
@@ -375,7 +378,7 @@ def test_gemm(M, N, K, dtype, out_dtype, how):
             assert (out[:, :odd] == 3).all() and (out[:, odd + cols:] == 3).all()
 
 
-@pytest.mark.parametrize("M,N,K,how", [(1540, 8208, 8192, "silu"), (1600, 8200, 8192, "add"), (700, 8300, 640, "store"), (260, 28672, 96, "silu")])
+@pytest.mark.parametrize("M,N,K,how", [(1540, 8208, 8192, "silu"), (1600, 8200, 8192, "add"), (1536, 2064, 2048, "silu"), (770, 4100, 4128, "store"), (700, 8300, 640, "store"), (260, 28672, 96, "silu")])
 def test_gemm_of_many_rows(M, N, K, how):
     """Through the weights' values and in tiles, with the workspace and without it: of one size within rounding."""
     from glassbox_amd import ops
