@@ -554,7 +554,7 @@ template <typename T, int NB> static void launch(const Plan& p, const AttendArgs
 
 using namespace gb;
 
-extern "C" int gb_fp4_attention_takes(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 256; }
+static bool takes(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 256; }
 
 // floats of workspace; 0: none is needed
 extern "C" long long gb_fp4_attention_floats(int n_seqs, int nh, int nkv, int hd, int max_q, int max_context, int window, int dtype) {
@@ -567,7 +567,7 @@ extern "C" int gb_fp4_attention(const void* q, int q_stride, void* out, int out_
                                 const int32_t* q_len, const int32_t* pos0, int n_seqs, int max_q, int max_context, const int32_t* tables,
                                 int table_stride, int table_cols, const void* k_pages, const void* v_pages, int pages, int nh, int nkv, int hd,
                                 int page, float scale, int window, float* workspace, long long workspace_floats, hipStream_t stream) {
-  GB_REQUIRE(gb_fp4_attention_takes(hd), "fp4_attention: heads of %d channels: 32, 64, 96, 128 or 256", hd);
+  GB_REQUIRE(takes(hd), "fp4_attention: heads of %d channels: 32, 64, 96, 128 or 256", hd);
   GB_REQUIRE(n >= 0 && n_seqs >= 0 && nkv > 0 && nh > 0 && nh % nkv == 0, "fp4_attention: bad sizes n=%d requests=%d heads=%d/%d", n, n_seqs, nh, nkv);
   GB_REQUIRE(page > 0 && page % 16 == 0 && pages > 0 && table_cols > 0, "fp4_attention: pages of %d slots, %d pages, %d table columns", page, pages,
              table_cols);

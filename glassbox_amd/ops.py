@@ -288,7 +288,6 @@ _SIGS = {
         "gb_fp4_attention": [_vp, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _i,
                              _vp, C.c_longlong, _vp],
         "gb_fp4_attention_floats": [_i, _i, _i, _i, _i, _i, _i, _i],
-        "gb_fp4_attention_takes": [_i],
     },
     "fp4_gemm": {
         # a, dtype, lda, codes, scales, scales a row, out, its dtype, ldo, M, N, K, epilogue, workspace, its floats, stream
