@@ -417,9 +417,9 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least
 }
 
 // More columns: each of four waves has R tiles of its own and takes all keys.  Bound by the conversions and the softmax: 2,048 rows of 32 heads of
-// 128 in 64 us (the same rows over a bf16 cache in the prefill kernel: 56).  A request's long tiles of columns come first and its short ones
-// behind them in turn, so that compute units of two workgroups have about the same to do: in their order 84.  Making a tile bf16 once for the four waves, through LDS, took 95: the barriers cost more than the
-// conversions that they save.
+// 128 in 62 us (the same rows over a bf16 cache in the prefill kernel: 56).  A request's long tiles of columns come first and its short ones
+// behind them in turn, so that compute units of two workgroups have about the same to do: in their order 84.  Making a tile bf16 once for the
+// four waves, through LDS, took 95: the barriers cost more than the conversions that they save.
 template <typename T, int NB, int R>
 __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(least_waves<T, NB, R>))) void fp4_attend_cols_kernel(AttendArgs a) {
   constexpr int D = NB * kFp4Block, C = 16 * R;
@@ -518,7 +518,7 @@ static Plan plan(int n_seqs, int nkv, int rep, int hd, int max_q, int max_contex
   Plan p;
   const long long columns = (long long)max_q * rep;
   p.cols = columns > 32;
-  // Waves with columns of their own: two tiles of them where there is much to do and they fit the registers (2,048 rows of 32 heads of 128: 64 us,
+  // Waves with columns of their own: two tiles of them where there is much to do and they fit the registers (2,048 rows of 32 heads of 128: 62 us,
   // one tile 89; 131 rows behind 3,900: 29.1 and 30.9; 120 rows of 5 requests, 3 heads a kv head: 7.7 and 5.9).
   const long long longest = window > 0 ? std::min(max_context, window) : max_context;
   p.r = p.cols && (columns >= 1024 || (columns >= 128 && longest >= 2048)) && dtype == kBF16 && hd <= 128 ? 2 : 1;
