@@ -88,11 +88,14 @@ template <typename T> __device__ __forceinline__ void store4(T* p, bool wide, co
 struct Places {
   int kp, vp, koff, voff;
 };
-__device__ __forceinline__ Places look_up(const AttendArgs& a, const int32_t* table, int kt, int vt) {
-  const int ki = a.page_shift >= 0 ? kt >> a.page_shift : kt / a.page, vi = a.page_shift >= 0 ? vt >> a.page_shift : vt / a.page;
-  const int k0 = table[min(ki, a.table_cols - 1)], v0 = table[min(vi, a.table_cols - 1)];
-  return {ki < a.table_cols ? k0 : -1, vi < a.table_cols ? v0 : -1, kt - ki * a.page, vt - vi * a.page};
+__device__ __forceinline__ Places look_up(const AttendArgs& a, const int32_t* table, uint32_t kt, uint32_t vt) {
+  const uint32_t page = a.page, columns = a.table_cols;   // (whatever the tokens' numbers, what is read lies in the table)
+  const uint32_t ki = a.page_shift >= 0 ? kt >> a.page_shift : kt / page, vi = a.page_shift >= 0 ? vt >> a.page_shift : vt / page;
+  const int k0 = table[min(ki, columns - 1)], v0 = table[min(vi, columns - 1)];
+  return {ki < columns ? k0 : -1, vi < columns ? v0 : -1, (int)(kt - ki * page), (int)(vt - vi * page)};
 }
+// the first key that a window leaves a position; no sum passes 32 bits, whatever the position
+__device__ __forceinline__ int window_from(const AttendArgs& a, int pos) { return a.window > 0 ? max(pos, a.window - 1) - (a.window - 1) : 0; }
 // a page of the pool; page 0 in the place of any other number, which is not read
 __device__ __forceinline__ bool known_page(const AttendArgs& a, int page) { return (unsigned)page < (unsigned)a.pages; }
 __device__ __forceinline__ size_t page_at(const AttendArgs& a, int page, int kvh, size_t head_bytes) {
@@ -257,7 +260,7 @@ template <typename T, int NB, int R> struct Columns {
     for (int t = 0; t < R; ++t) {
       const int c = min(c0 + 16 * t + r, cols - 1);
       pos[t] = pos0 + c / a.rep;
-      from[t] = a.window > 0 ? pos[t] - a.window + 1 : 0;
+      from[t] = window_from(a, pos[t]);
       load_query<T, NB>((const T*)a.q + (size_t)(q_start + c / a.rep) * a.q_stride + (size_t)(kvh * a.rep + c % a.rep) * (NB * kFp4Block), g, a.q_wide, qf[t]);
       m[t] = -__builtin_inff();
       l[t] = 0.f;
@@ -356,12 +359,12 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least
   id /= a.col_tiles;
   const int split = id % a.splits, s = id / a.splits;
 
-  const int q_start = a.q_start[s], pos0 = a.pos0[s];
+  const int q_start = a.q_start[s], pos0 = min(a.pos0[s], INT32_MAX - a.max_q);
   const int cols = q_start < 0 ? 0 : min(min(a.q_len[s], a.max_q), a.n - q_start) * a.rep;
   if (c0 >= cols) return;   // (the whole workgroup)
   const int first = pos0 + c0 / a.rep, last = pos0 + min(cols - 1, c0 + 15) / a.rep;   // positions of the columns
-  const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0, begin = (lo & ~(kTile - 1)) + split * a.chunk;
-  const int end = min(min(last + 1, a.table_cols * a.page), begin + a.chunk);
+  const int limit = max(0, min(last + 1, a.table_cols * a.page)), lo = min(window_from(a, first), limit);
+  const int begin = (int)min((long long)(lo & ~(kTile - 1)) + (long long)split * a.chunk, (long long)limit), end = begin + min(limit - begin, a.chunk);
 
   // the numbers of a tile's pages are asked for a tile ahead, those of the first before the queries
   const int32_t* table = a.tables + (size_t)s * a.table_stride;
@@ -434,13 +437,13 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(least
   id /= a.col_tiles;
   const int split = id % a.splits, s = id / a.splits;
 
-  const int q_start = a.q_start[s], pos0 = a.pos0[s];
+  const int q_start = a.q_start[s], pos0 = min(a.pos0[s], INT32_MAX - a.max_q);
   const int cols = q_start < 0 ? 0 : min(min(a.q_len[s], a.max_q), a.n - q_start) * a.rep;
   const int c0 = (col_tile * 4 + wave) * C;
   if (c0 >= cols) return;   // (the wave: there is no barrier)
   const int first = pos0 + c0 / a.rep, last = pos0 + min(cols - 1, c0 + C - 1) / a.rep;   // positions of the wave's columns
-  const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0, begin = (lo & ~(kTile - 1)) + split * a.chunk;
-  const int end = min(min(last + 1, a.table_cols * a.page), begin + a.chunk);
+  const int limit = max(0, min(last + 1, a.table_cols * a.page)), lo = min(window_from(a, first), limit);
+  const int begin = (int)min((long long)(lo & ~(kTile - 1)) + (long long)split * a.chunk, (long long)limit), end = begin + min(limit - begin, a.chunk);
 
   const int32_t* table = a.tables + (size_t)s * a.table_stride;
   Places at = look_up(a, table, begin + 16 * (r >> 2), begin + 16 * g);
@@ -532,7 +535,7 @@ static Plan plan(int n_seqs, int nkv, int rep, int hd, int max_q, int max_contex
   const long long groups = (long long)n_seqs * nkv * p.col_tiles;
   const long long want = ((p.cols ? 512 : 256) + groups / 2) / groups, least = p.cols ? 256 : 1024, grain = p.cols ? kTile : 8 * kTile;
   const long long runs = std::max<long long>(1, std::min<long long>(want, kMostSplits));
-  const long long chunk = std::max(least, ((span + runs - 1) / runs + grain - 1) / grain * grain);
+  const long long chunk = std::min<long long>(std::max(least, ((span + runs - 1) / runs + grain - 1) / grain * grain), 1 << 30);
   p.splits = (int)std::max<long long>(1, (span + chunk - 1) / chunk);
   p.chunk = (int)chunk;
   return p;
@@ -574,7 +577,7 @@ extern "C" int gb_fp4_attention(const void* q, int q_stride, void* out, int out_
   GB_REQUIRE((long long)nh * hd <= q_stride && (long long)nh * hd <= out_stride, "fp4_attention: row strides %d, %d are shorter than the heads", q_stride,
              out_stride);
   GB_REQUIRE(dtype == kF32 || dtype == kBF16, "fp4_attention: unknown dtype %d", dtype);
-  GB_REQUIRE(max_q >= 0 && max_context >= 0 && (long long)table_cols * page < (1ll << 31), "fp4_attention: rows %d, context %d, tables of %d pages", max_q,
+  GB_REQUIRE(max_q >= 0 && max_context >= 0 && (long long)table_cols * page <= INT32_MAX - 1024, "fp4_attention: rows %d, context %d, tables of %d pages", max_q,
              max_context, table_cols);
   if (n == 0 || n_seqs == 0 || max_q == 0) return 0;
   const int rep = nh / nkv;

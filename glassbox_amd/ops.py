@@ -2718,8 +2718,8 @@ def fp4_attention(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_l
         raise KernelError(f"fp4_attention: q and out must be [n, {n_heads} heads * {hd}] of one type")
     if hd not in FP4_HEAD_DIMS or n_heads <= 0 or n_heads % nkv:
         raise KernelError(f"fp4_attention: {n_heads} query heads of {hd} channels over {nkv} kv heads: heads of {FP4_HEAD_DIMS}, a multiple of the kv heads")
-    if not 0 < scale < math.inf:
-        raise KernelError(f"fp4_attention: a positive scale is needed, got {scale}")
+    if not 1e-30 < scale < 1e30:
+        raise KernelError(f"fp4_attention: a positive scale (1e-30 to 1e30) is needed, got {scale}")
     seqs = q_len.numel()
     _i32(q_start, "q_start", seqs)
     _i32(q_len, "q_len", seqs)
@@ -2794,7 +2794,7 @@ def _fp4_expands(rows: int, n: int, k: int, dtype: torch.dtype, out_dtype: torch
     kernel that converts on the way, and more than the values cost: 2,048 rows by 28,672 of 4,096 428 and 537, by 6,144 of 2,048 51 and 69;
     768 by 4,096 of 14,336 115 and 153.  Not so for fewer rows (512 by 4,096 of 14,336 93 and 87) or numbers (2,048 by 1,600 of 960 20 and 15)."""
     size = n * k
-    return (dtype == torch.bfloat16 and (rows >= 1536 and size >= 1 << 22 or rows >= 768 and size >= 1 << 24)
+    return (dtype == torch.bfloat16 and (1536 <= rows <= 1 << 20 and size >= 1 << 22 or 768 <= rows < 1536 and size >= 1 << 24)
             and not (silu_mul and (n % 16 or out_dtype != torch.bfloat16)))
 
 

@@ -56,7 +56,7 @@ REFUSED = [
     (attention, dict(q=torch.zeros(5, 192, dtype=BF), out=torch.zeros(5, 192, dtype=BF), H=3), "multiple of the kv heads"),
     (attention, dict(q=torch.zeros(5, 640, dtype=BF), out=torch.zeros(5, 640, dtype=BF), k=pages(d=160), v=pages(d=160)), "heads of"),
     (attention, dict(scale=0.0), "positive"), (attention, dict(scale=-1.0), "positive"), (attention, dict(scale=math.nan), "positive"),
-    (attention, dict(scale=math.inf), "positive"), (attention, dict(pos0=torch.zeros(1, dtype=I32)), "pos0"),
+    (attention, dict(scale=math.inf), "positive"), (attention, dict(scale=1e-40), "positive"), (attention, dict(pos0=torch.zeros(1, dtype=I32)), "pos0"),
     (attention, dict(q_start=torch.zeros(2)), "q_start"), (attention, dict(tables=torch.zeros(1, 4, dtype=I32)), "tables"),
     (attention, dict(tables=torch.zeros(2, 0, dtype=I32)), "tables"), (attention, dict(tables=torch.zeros(4, 2, dtype=I32).t()), "tables"),
     (attention, dict(window=-1), "below 0"), (attention, dict(most=-1), "below 0"), (attention, dict(ws=torch.zeros(8, dtype=BF)), "workspace"),

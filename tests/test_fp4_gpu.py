@@ -520,3 +520,55 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for out, want in zip(outs, wants):
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_with_the_loosest_bound_of_the_contexts(dtype, rows, window):
+    """``max_context`` as large as it may be: more runs than there are keys, the answer of any other bound."""
+    kp, vp, tables = cached([rows + 130, rows + 7], 2, 64, 16, 50)
+    q = normal(2 * rows, 4 * 64, seed=51).to(dtype)
+    for many in (1, 300):                                  # few requests, whose contexts are divided, and more than compute units
+        start, length, pos0 = [0, rows] + [0] * (2 * many - 2), [rows, rows] + [0] * (2 * many - 2), [130, 7] + [0] * (2 * many - 2)
+        table = tables.repeat(many, 1)
+        got = attend(q.to(DEV), start, length, pos0, table.to(DEV), kp.to(DEV), vp.to(DEV), 4, 0.1, window, max_context=2 ** 31 - 1)
+        check(got, q, [0, rows], [rows, rows], [130, 7], tables, kp, vp, 4, 0.1, window)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_at_positions_that_no_table_has(dtype, rows):
+    """Positions at the ends of 32 bits: with a window such rows see nothing and give zeros, without one all that the table has, from behind; those
+    before the first key see nothing."""
+    kp, vp, tables = cached([64], 2, 64, 16, 52)
+    q = normal(rows, 4 * 64, seed=53).to(dtype)
+    k, v, t = kp.to(DEV), vp.to(DEV), tables.to(DEV)
+    every = attend(q.to(DEV), [0], [rows], [64], t, k, v, 4, 0.1, max_context=200)
+    check(every, q, [0], [rows], [64], tables, kp, vp, 4, 0.1)
+    for pos0 in (2 ** 31 - 1, 2 ** 31 - 60, 2 ** 30):
+        far = attend(q.to(DEV), [0], [rows], [pos0], t, k, v, 4, 0.1, max_context=200)
+        assert torch.equal(far, every)
+        for window in (1, 64, 2 ** 31 - 1 - 2 ** 30 - 100):
+            assert (attend(q.to(DEV), [0], [rows], [pos0], t, k, v, 4, 0.1, window, max_context=200) == 0).all()
+    for pos0 in (-rows, -(2 ** 31) + rows):
+        for window in (0, 1, 2 ** 31 - 1):
+            assert (attend(q.to(DEV), [0], [rows], [pos0], t, k, v, 4, 0.1, window, max_context=200) == 0).all()
+
+
+@pytest.mark.parametrize("how", ["silu", "add", "store"])
+def test_gemm_through_the_values_into_rows_that_begin_anywhere(how):
+    from glassbox_amd import ops
+    M, N, K = 1537, 2064, 2048
+    w = ops.fp4_quantize(normal(N, K, seed=54, scale=0.05).to(DEV))
+    a = normal(M, K, seed=55).bfloat16().to(DEV)
+    dtype, cols = (torch.float32, N) if how == "add" else (torch.bfloat16, N // 2 if how == "silu" else N)
+    floats = ops.fp4_gemm_floats(M, N, K, torch.bfloat16, dtype, how == "silu")
+    assert floats >= N * K // 2
+    outs = []
+    for odd in (0, 3):
+        out = torch.full((M, cols + 2 * odd), 2.0, dtype=dtype, device=DEV)
+        ops.fp4_gemm(a, w, out[:, odd:odd + cols], accumulate=how == "add", silu_mul=how == "silu", workspace=torch.empty(floats, device=DEV))
+        assert not odd or ((out[:, :odd] == 2).all() and (out[:, odd + cols:] == 2).all())
+        outs.append(out[:, odd:odd + cols])
+    assert torch.equal(outs[0], outs[1])
