@@ -108,7 +108,7 @@ class Engine:
     kv_cache: None, keys and values in the compute type; "fp4", in blocks of 32 four-bit numbers that share a power of two
     (``ops.fp4_store``, ``ops.fp4_attention``): 4.25 bits a number, 3.76 times the tokens in the memory of a bfloat16 cache.
     weights: None, the layers' matrices in the compute type; "fp4", in such blocks, the nearest (``ops.fp4_gemm``); the embedding
-    and the head stay as they are.  A loaded model that is handed in is quantized in place.
+    and the head stay as they are.  A loaded model that is handed in is quantized in place.  These kernels are the same whatever ``kernels``.
     """
 
     def __init__(self, model, dtype="bfloat16", max_tokens: int = 4096, max_seqs: int = 32, page_size: int = 16,

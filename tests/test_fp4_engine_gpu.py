@@ -168,3 +168,56 @@ def test_the_command_line(model_dirs):
     assert r.returncode == 0, r.stderr
     eng = Engine(folder, dtype="float32", max_tokens=64, max_seqs=1, kv_cache="fp4", weights="fp4")
     assert [int(t) for t in r.stdout.split()] == greedy(eng, [5, 17, 3, 300, 41], 8)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_window_and_a_layer_that_reads_another_ones_cache(packed):
+    """Three layers: all keys; the last twenty, whose pages are given back on the way; the first layer's cache, read alone."""
+    from glassbox_amd.config import config_from_dict
+    from glassbox_amd.engine import Engine
+    from glassbox_amd.parts.attention import PagedAttention
+    from glassbox_amd.parts.block import PreNormBlock
+    from glassbox_amd.parts.embedding import Embedding, LMHead
+    from glassbox_amd.parts.mlp import SwiGLU
+    from glassbox_amd.parts.model import DecoderModel, LayerCall
+    from glassbox_amd.parts.norm import RMSNorm
+    from glassbox_amd.parts.rotary import Rotary
+    from glassbox_amd.weights.loader import random_tensors
+    d, H, G, D, vocab, eps, theta, window = 96, 6, 2, 64, 90, 1e-5, 10000.0, 20
+    rotary = Rotary(D, theta)
+    layer = lambda **how: PreNormBlock(RMSNorm(d, eps), PagedAttention(d, H, G, D, rotary, **how), RMSNorm(d, eps), SwiGLU(d, 160))
+    embedding = Embedding(vocab, d)
+    cfg = config_from_dict(dict(helpers.TINY_B, hidden_size=d, intermediate_size=160, num_hidden_layers=3, num_attention_heads=H,
+                                num_key_value_heads=G, head_dim=D, vocab_size=vocab, rope_theta=theta, rms_norm_eps=eps, tie_word_embeddings=True))
+    model = DecoderModel(cfg, embedding, [layer(), layer(window=window), layer(shares_kv=True)],
+                         [LayerCall(0, cache=0), LayerCall(1, cache=1), LayerCall(2, reads=0)], RMSNorm(d, eps), LMHead(vocab, d, tied_to=embedding))
+    tensors = random_tensors(model, 7, 0.1, "uniform", torch.float32, "cuda:0")
+    model.load_tree(tensors)
+    w = {n: t.cpu() for n, t in tensors.items()}
+    w = {n: (fp4_plain.rounded(t) if packed and n.startswith("model.layers.") and t.dim() == 2 else t).double() for n, t in w.items()}
+    eng = Engine(model, dtype="float32", max_tokens=256, max_seqs=2, kv_cache="fp4", weights="fp4" if packed else None)
+    assert len(eng.group_keys) == 2
+    tokens, held, got, at = helpers.random_tokens(vocab, 70, 8), {0: [], 1: []}, [], 0
+    for n in (16, 13, 1, 16, 9) + (1,) * 15:
+        got.extend(eng.step([("r", tokens[at:at + n], list(range(n)))]).cpu().numpy())
+        at += n
+        for c, kept in held.items():      # (what this step brought: the window's pages go back later)
+            lc, sid = eng.layers[c], eng._ids["r"]
+            k_pages, v_pages = lc.k_pages.cpu(), lc.v_pages.cpu()
+            kept += [fp4_plain.get(k_pages, v_pages, eng.cache.slot(sid, t, lc.group)) for t in range(at - n, at)]
+    assert at == 70 and eng.cache.table(eng._ids["r"], 1)[:2] == [-1, -1]
+    x = w["model.embed_tokens.weight"][torch.tensor(tokens)]
+    for li, (source, seen) in enumerate(((0, 0), (1, window), (0, 0))):
+        p = f"model.layers.{li}."
+        h = plain.rms_norm(x, w[p + "input_layernorm.weight"], eps)
+        k, v = (torch.stack(t) for t in zip(*held[source]))
+        if li < 2:
+            made_k, made_v = ((h @ w[p + f"self_attn.{n}_proj.weight"].T).reshape(70, G, D) for n in "kv")
+            assert nearest(k, plain.rope(made_k, range(70), theta), 1e-4).all() and nearest(v, made_v, 1e-4).all()
+        q = plain.rope((h @ w[p + "self_attn.q_proj.weight"].T).reshape(70, H, D), range(70), theta)
+        x = x + plain.attention(q, k, v, seen).reshape(70, H * D) @ w[p + "self_attn.o_proj.weight"].T
+        h = plain.rms_norm(x, w[p + "post_attention_layernorm.weight"], eps)
+        x = x + plain.swiglu(h, *(w[p + f"mlp.{n}_proj.weight"] for n in ("gate", "up", "down")))
+    want = (plain.rms_norm(x, w["model.norm.weight"], eps) @ w["model.embed_tokens.weight"].T).numpy()
+    bad = helpers.first_bad(np.asarray(got), want, helpers.TOL_F32)
+    assert bad is None, f"position {bad[0]} off by {bad[1]:.3e}"
