@@ -21,6 +21,7 @@
 #include "fp4.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace gb {
 
@@ -518,27 +519,49 @@ struct Plan {
 
 // How a launch is laid out: a function of its sizes and the rows' type alone.
 static Plan plan(int n_seqs, int nkv, int rep, int hd, int max_q, int max_context, int window, int dtype) {
-  Plan p;
   const long long columns = (long long)max_q * rep;
-  p.cols = columns > 32;
-  // Waves with columns of their own: two tiles of them where there is much to do and they fit the registers (2,048 rows of 32 heads of 128: 62 us,
-  // one tile 89; 131 rows behind 3,900: 29.1 and 30.9; 120 rows of 5 requests, 3 heads a kv head: 7.7 and 5.9).
-  const long long longest = window > 0 ? std::min(max_context, window) : max_context;
-  p.r = p.cols && (columns >= 1024 || (columns >= 128 && longest >= 2048)) && dtype == kBF16 && hd <= 128 ? 2 : 1;
-  const int width = p.cols ? 64 * p.r : 16;   // columns a workgroup
-  p.col_tiles = (int)((columns + width - 1) / width);
-  const long long tokens = std::min<long long>(max_q, (16 * p.r - 1) / rep + 2);   // of a wave's columns
-  const long long span = window > 0 ? std::min<long long>(max_context, window + tokens + kTile) : max_context;
-  // Runs of a context: about as many workgroups as compute units (half as many again of four waves), none of fewer than 1,024 keys (256).  us:
-  // 4 requests of 16,000 keys and 8 kv heads in 8 runs 23.6, in 4 29.6, in 16 28.7; 256 workgroups in one run 18.2, in two 21.9; 131 rows behind
-  // 3,900, 32 heads, in 8 30, in 4 34.
-  const long long groups = (long long)n_seqs * nkv * p.col_tiles;
-  const long long want = ((p.cols ? 512 : 256) + groups / 2) / groups, least = p.cols ? 256 : 1024, grain = p.cols ? kTile : 8 * kTile;
-  const long long runs = std::max<long long>(1, std::min<long long>(want, kMostSplits));
-  const long long chunk = std::min<long long>(std::max(least, ((span + runs - 1) / runs + grain - 1) / grain * grain), 1 << 30);
-  p.splits = (int)std::max<long long>(1, (span + chunk - 1) / chunk);
-  p.chunk = (int)chunk;
-  return p;
+  auto laid_out = [&](bool cols, int r, long long runs, long long least, long long grain) {
+    const int width = cols ? 64 * r : 16;   // columns a workgroup
+    const long long tokens = std::min<long long>(max_q, (16 * r - 1) / rep + 2);   // of a wave's columns
+    const long long span = window > 0 ? std::min<long long>(max_context, window + tokens + kTile) : max_context;
+    const long long chunk = std::min<long long>(std::max(least, ((span + runs - 1) / runs + grain - 1) / grain * grain), 1 << 30);
+    return Plan{cols, r, (int)((columns + width - 1) / width), (int)std::max<long long>(1, (span + chunk - 1) / chunk), (int)chunk};
+  };
+  // Few columns, runs of a context: as many workgroups as compute units have one, none of fewer than 512 keys; 129 to 217 workgroups of long contexts
+  // in three.  Over 110 sizes 1.6 % slower than the best number of runs.  us: one request of 4,000 keys and 32 kv heads in 8 runs 9.5, in 4 11;
+  // 256 workgroups in one run 18.2, in two 21.9; 160 (5 of 9,000) in three 28.4, in two 35.5.  More than 256 stay whole: 40 requests of 1,000 to 8,000 keys
+  // and 8 kv heads 61.6, in three 65.4, though 10 of 9,000 and 32 kv heads take 58 and 47.
+  if (columns <= 32) {
+    const long long groups = (long long)n_seqs * nkv * ((columns + 15) / 16);
+    long long runs = std::max<long long>(1, std::min<long long>(256 / groups, kMostSplits));
+    if (groups > 128 && groups < 218 && max_context >= 4096) runs = 3;
+    if (max_context <= 1024) runs = 1;
+    return laid_out(false, 1, runs, 512, 8 * kTile);
+  }
+  // More: one tile of columns a wave or two (where they fit the registers), and as many runs, as take least by a model with numbers fitted to 1,900 launches
+  // (70 sizes, 9 % off; its choice is 2.5 % slower than the best, at most 18): a wave's turns, each `alone` us; the tiles that a SIMD has to do on
+  // average, `busy` us each, more where the workgroups do not divide evenly by the compute units; the joining of runs, its launch and its
+  // bytes.  us: 131 rows behind 3,900, 32 heads of 64 and as many kv heads, two tiles in 8 runs 28.4, in 5 31.9, one tile in 8 30.2; 8 kv heads of 128 two
+  // in 6 33.4, in 8 38.6; 1,024 rows of 32 heads of 64 two in one run 23, in two 43; 8 x 50 rows behind 550 one in one 16, two in three 25.
+  static constexpr float kAlone[2][9] = {{0.f, 0.4f, 0.55f, 1.2f, 0.75f, 0.f, 0.f, 0.f, 1.f}, {0.f, 0.55f, 0.65f, 1.35f, 1.05f}};   // by tiles and blocks a head
+  static constexpr float kBusy[2][9] = {{0.f, 0.55f, 0.65f, 1.1f, 0.83f, 0.f, 0.f, 0.f, 2.2f}, {0.f, 0.62f, 0.84f, 1.2f, 0.91f}};
+  const bool wide = dtype == kF32;
+  Plan best{};
+  float least = 0.f;
+  for (int r = 1; r <= (!wide && hd <= 128 ? 2 : 1); ++r) {
+    const float alone = kAlone[r - 1][hd / 32] * (wide ? 1.25f : 1.f), busy = kBusy[r - 1][hd / 32] * (wide ? 1.65f : 1.f);
+    const float waves = (float)n_seqs * nkv * (float)((columns + 16 * r - 1) / (16 * r));
+    for (int runs : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64}) {
+      const Plan p = laid_out(true, r, runs, kTile, kTile);
+      const float groups = (float)n_seqs * nkv * p.col_tiles * p.splits / 256, span = std::min((float)max_context, (float)p.chunk * p.splits);
+      if (runs > 1 && groups > 32) break;
+      const float seen = window > 0 ? span : std::max(span - max_q / 2.f, span / 2);   // keys of a row, on average
+      float us = p.chunk / 64.f * alone + waves * seen / 64 / 1024 * busy * (1 + 0.6f * (std::ceil(groups) / groups - 1));
+      if (p.splits > 1) us += 2.5f + (float)n_seqs * max_q * nkv * rep * (hd + 2) * p.splits / 500e3f;
+      if (best.splits == 0 || us < least) least = us, best = p;
+    }
+  }
+  return best;
 }
 
 template <typename T, int NB> static void launch(const Plan& p, const AttendArgs& a, int n_seqs, hipStream_t stream) {
