@@ -496,9 +496,10 @@ def _p(t: Optional[torch.Tensor]):
 
 def _rows(t: torch.Tensor, what: str) -> int:
     """Row stride of a 2-d tensor whose rows are dense."""
-    if t.dim() != 2 or t.stride(1) != 1:
-        raise KernelError(f"{what} must be 2-d with dense rows, got shape {tuple(t.shape)} strides {t.stride()}")
-    return t.stride(0)
+    step = t.stride()   # (one call for all of it: a step of short kernels is made of such calls)
+    if len(step) != 2 or step[1] != 1:
+        raise KernelError(f"{what} must be 2-d with dense rows, got shape {tuple(t.shape)} strides {step}")
+    return step[0]
 
 
 def _i32(t: Optional[torch.Tensor], what: str, n: Optional[int] = None) -> None:
@@ -2574,6 +2575,7 @@ def delta_chunk_floats(rows: int, n_seqs: int, n_heads: int, key_dim: int, value
 # 4, 6 times that (csrc/hip/fp4.h): 4.25 bits a number.  They hold keys and values of a cache (blocks of a head's channels) and
 # matrices (blocks of the inner size).  A block with a number that is infinite or NaN reads as NaN.
 FP4_BLOCK = 32
+_FLOAT, _BYTE, _INT = torch.float32, torch.uint8, torch.int32
 FP4_HEAD_DIMS = (32, 64, 96, 128, 256)   # heads that ``fp4_attention`` takes
 
 
@@ -2588,14 +2590,20 @@ class Fp4Matrix(NamedTuple):
         return self.codes.shape[0], 2 * self.codes.shape[1]
 
 
-def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """The operands lie on the current device, whose stream the kernels are launched on."""
-    here = None
-    for t in tensors:
-        if t is not None:
-            at = t.get_device()   # (-1: not on a GPU)
-            if at < 0 or at != (here := _get_device() if here is None else here):
-                raise KernelError(f"{what}: operands must be on the current GPU")
+def _here(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The current device, on whose stream the kernels are launched: the operands lie there."""
+    here = first.get_device()   # (-1: not on a GPU)
+    if here >= 0 and here == _get_device():
+        for t in others:
+            if t is not None and t.get_device() != here:
+                break
+        else:
+            return here
+    raise KernelError(f"{what}: operands must be on the current GPU")
+
+
+def _stream_of(device: int):
+    return _raw_stream(device) if _raw_stream is not None else _stream()
 
 
 def _apart(a0: int, a_rows: int, a_bytes: int, a_step: int, b0: int, b_rows: int, b_bytes: int, b_step: int) -> bool:
@@ -2619,8 +2627,8 @@ def _fp4_pages(k_pages, v_pages, what: str):
     """(pages, kv heads, page size, head size, where the keys' and the values' begin) of four-bit pages."""
     if k_pages is not None and v_pages is not None:
         shape, k_at, v_at = k_pages.shape, k_pages.data_ptr(), v_pages.data_ptr()
-        if (len(shape) == 5 and v_pages.shape == shape and shape[3] == 17 and shape[4] % 16 == 0 and k_pages.dtype == torch.uint8
-                and v_pages.dtype == torch.uint8 and k_pages.is_contiguous() and v_pages.is_contiguous() and (k_at | v_at) % 16 == 0):
+        if (len(shape) == 5 and v_pages.shape == shape and shape[3] == 17 and shape[4] % 16 == 0 and k_pages.dtype is _BYTE
+                and v_pages.dtype is _BYTE and k_pages.is_contiguous() and v_pages.is_contiguous() and (k_at | v_at) % 16 == 0):
             p, h, nb, _, s = shape
             if p and h and nb and s:
                 return p, h, s, nb * FP4_BLOCK, k_at, v_at
@@ -2653,7 +2661,7 @@ def fp4_store(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torc
     if cos is not None and sin is not None:
         for t in (cos, sin):
             shape = t.shape
-            if t.dtype != torch.float32 or not t.is_contiguous() or len(shape) != 2 or shape[0] < n or shape[1] != head_dim // 2:
+            if t.dtype is not _FLOAT or not t.is_contiguous() or len(shape) != 2 or shape[0] < n or shape[1] != head_dim // 2:
                 raise KernelError("fp4_store: cos/sin must be contiguous float32 [n, head_dim/2]")
         cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
     elif cos is not None or sin is not None:
@@ -2668,10 +2676,10 @@ def fp4_store(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torc
     at, q_at, e = qkv.data_ptr(), q.data_ptr(), 4 if dtype == F32 else 2
     if not (at == q_at and stride == q_stride) and n and n_heads and not _apart(q_at, n, n_heads * head_dim * e, q_stride * e, at, n, given * e, stride * e):
         raise KernelError("fp4_store: q lies over other columns of the rows")
-    _here("fp4_store", qkv, cos, sin, slots, k_pages, v_pages, q)
+    here = _here("fp4_store", qkv, cos, sin, slots, k_pages, v_pages, None if q is qkv else q)
     lib = _lib("fp4_cache")
     _launch(lib, lib.gb_fp4_store, at, dtype, stride, q_at, q_stride, cos_at, sin_at, slots_at, k_at, v_at, n, n_heads,
-            n_kv_heads, head_dim, page_size, pages, _stream())
+            n_kv_heads, head_dim, page_size, pages, _stream_of(here))
 
 
 def fp4_load(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -2686,10 +2694,10 @@ def fp4_load(slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     k_to, v_to, e = k.data_ptr(), v.data_ptr(), 4 if dtype == F32 else 2
     if n and not _apart(k_to, n, nkv * hd * e, k_stride * e, v_to, n, nkv * hd * e, v_stride * e):
         raise KernelError("fp4_load: k and v share memory")
-    _here("fp4_load", slots, k_pages, v_pages, k, v)
+    here = _here("fp4_load", slots, k_pages, v_pages, k, v)
     lib = _lib("fp4_cache")
     _launch(lib, lib.gb_fp4_load, slots.data_ptr(), k_at, v_at, k_to, k_stride, v_to, v_stride, dtype, n, nkv, hd, page_size,
-            pages, _stream())
+            pages, _stream_of(here))
 
 
 @functools.lru_cache(maxsize=4096)   # a pure function of the sizes, asked for at every step
@@ -2721,11 +2729,13 @@ def fp4_attention(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_l
     if not 1e-30 < scale < 1e30:
         raise KernelError(f"fp4_attention: a positive scale (1e-30 to 1e30) is needed, got {scale}")
     seqs = q_len.numel()
-    _i32(q_start, "q_start", seqs)
-    _i32(q_len, "q_len", seqs)
-    _i32(pos0, "pos0", seqs)
+    if not (q_start.dtype is _INT and q_len.dtype is _INT and pos0.dtype is _INT and q_start.is_contiguous() and q_len.is_contiguous()
+            and pos0.is_contiguous() and q_start.numel() >= seqs and pos0.numel() >= seqs):
+        for t, name in ((q_start, "q_start"), (q_len, "q_len"), (pos0, "pos0")):
+            _i32(t, name, seqs)
     tables_shape = tables.shape
-    if tables.dtype != torch.int32 or len(tables_shape) != 2 or tables.stride(1) != 1 or tables_shape[0] < seqs or tables_shape[1] == 0:
+    tables_step = tables.stride()
+    if tables.dtype is not _INT or len(tables_shape) != 2 or tables_step[1] != 1 or tables_shape[0] < seqs or tables_shape[1] == 0:
         raise KernelError("fp4_attention: block tables must be int32 [requests, pages]")
     window, max_q_len, max_context = int(window), int(max_q_len), int(max_context)
     if not (0 <= window < 1 << 31 and 0 <= max_q_len < 1 << 31 and 0 <= max_context < 1 << 31):
@@ -2735,11 +2745,11 @@ def fp4_attention(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_l
     if not (at == to and q_stride == out_stride) and n and not _apart(at, n, shape[1] * e, q_stride * e, to, n, shape[1] * e, out_stride * e):
         raise KernelError("fp4_attention: out lies over other rows of q")
     ws_at, ws_floats = _fp4_workspace(workspace, "fp4_attention")
-    _here("fp4_attention", q, out, q_start, q_len, pos0, tables, k_pages, v_pages, workspace)
+    here = _here("fp4_attention", q, out, q_start, q_len, pos0, tables, k_pages, v_pages, workspace)
     lib = _lib("fp4_attention")
     _launch(lib, lib.gb_fp4_attention, at, q_stride, to, out_stride, dtype, n, q_start.data_ptr(), q_len.data_ptr(),
-            pos0.data_ptr(), seqs, max_q_len, max_context, tables.data_ptr(), tables.stride(0), tables_shape[1], k_at, v_at, pages, n_heads, nkv, hd,
-            page_size, scale, window, ws_at, ws_floats, _stream())
+            pos0.data_ptr(), seqs, max_q_len, max_context, tables.data_ptr(), tables_step[0], tables_shape[1], k_at, v_at, pages, n_heads, nkv, hd,
+            page_size, scale, window, ws_at, ws_floats, _stream_of(here))
 
 
 def _fp4_workspace(workspace: Optional[torch.Tensor], what: str) -> Tuple[Optional[int], int]:
@@ -2769,10 +2779,11 @@ def fp4_quantize(w: torch.Tensor) -> Fp4Matrix:
 def _fp4_matrix(w: Fp4Matrix, what: str) -> Tuple[int, int, int, int, int]:
     """(rows, columns, scales a row, where codes and scales begin) of a four-bit matrix."""
     codes, scales = w
-    if codes.dim() == 2 and scales.dim() == 2:
-        (n, half), (m, each), c_at, s_at = codes.shape, scales.shape, codes.data_ptr(), scales.data_ptr()
-        if (n > 0 and half > 0 and half % 16 == 0 and m == n and each == (half // 16 + 15) // 16 * 16 and codes.dtype == torch.uint8
-                and scales.dtype == torch.uint8 and codes.is_contiguous() and scales.is_contiguous() and (c_at | s_at) % 16 == 0):
+    codes_shape, scales_shape = codes.shape, scales.shape
+    if len(codes_shape) == 2 and len(scales_shape) == 2:
+        (n, half), (m, each), c_at, s_at = codes_shape, scales_shape, codes.data_ptr(), scales.data_ptr()
+        if (n > 0 and half > 0 and half % 16 == 0 and m == n and each == (half // 16 + 15) // 16 * 16 and codes.dtype is _BYTE
+                and scales.dtype is _BYTE and codes.is_contiguous() and scales.is_contiguous() and (c_at | s_at) % 16 == 0):
             return n, 2 * half, each, c_at, s_at
     raise KernelError(f"{what}: a four-bit matrix has contiguous uint8 codes [rows, columns / 2] and scales [rows, columns / 32 filled up to a "
                       f"multiple of 16], got {tuple(codes.shape)} and {tuple(scales.shape)}")
@@ -2829,7 +2840,7 @@ def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool 
     if M and not _apart(at, M, K * e, lda * e, to, M, (N // 2 if silu_mul else N) * f, ldo * f):
         raise KernelError("fp4_gemm: a and out share memory")
     ws_at, floats = _fp4_workspace(workspace, "fp4_gemm")
-    _here("fp4_gemm", a, w.codes, w.scales, out, workspace)
+    here = _here("fp4_gemm", a, w[0], w[1], out, workspace)
     if floats >= N * K // 2 and _fp4_expands(M, N, K, a.dtype, out.dtype, silu_mul) and lda % 8 == 0 and at % 16 == 0:
         values, rest = workspace[:N * K // 2].view(torch.bfloat16).view(N, K), workspace[N * K // 2:]
         fp4_expand(w, values)
@@ -2837,4 +2848,4 @@ def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool 
         return
     lib = _lib("fp4_gemm")
     _launch(lib, lib.gb_fp4_gemm, at, dtype, lda, c_at, s_at, each, to, out_dtype, ldo, M, N, K,
-            2 if silu_mul else 1 if accumulate else 0, ws_at, floats, _stream())
+            2 if silu_mul else 1 if accumulate else 0, ws_at, floats, _stream_of(here))
