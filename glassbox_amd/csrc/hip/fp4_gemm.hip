@@ -15,7 +15,8 @@
 //   compute unit, 20 to 50 GB/s each.)
 // Measured and left: workgroups that go on from tile to tile with the next one's lines under way (8 rows by 28,672 of 4,096 25.6, like this 22.7:
 // more registers, fewer waves); an RMS norm of the rows on the way (41, and 25.5 with the norm in a launch of its own: rows of 32 bits and
-// gamma are three times the bytes into every compute unit).
+// gamma are three times the bytes into every compute unit).  What a norm costs up to 8 rows, where the product before prepares it (gamma x in bf16 and
+// partial sums of squares) and this one divides by the root: 8 rows by 4,096 of 4,096, then by 28,672 31.4 us for both, 32.9 with a launch between.
 #include "fp4.h"
 
 #include <algorithm>
@@ -28,6 +29,14 @@ struct GemmArgs {
   const uint8_t *codes, *scales;
   void* out;
   float* slices;   // [slices, M, N]: given, each slice of k leaves its sums there
+  // Of RMS norms, up to 8 bf16 rows.  parts: the rows are bf16(gamma x) of an x whose squares' sums these are, [n_parts, 8], to be added up; h: the
+  // product adds into such an x, and writes bf16(gamma x) there and a tile's sums of squares to sums [n_tiles, 8].
+  const float* parts;
+  const void* gamma;
+  bf16* h;
+  float* sums;
+  int n_parts, gamma32, ldh;
+  float eps;
   int ldx, ldo, M, N, blocks, scale_stride, n_tiles, m_tiles, turns, epilogue, out32, out_wide;   // epilogue 0 store, 1 add, 2 silu(gate) * up
 };
 
@@ -82,8 +91,8 @@ __device__ __forceinline__ void terms_of(const Raw<float>& v, bf16x8 (&out)[3]) 
 }
 
 // T the rows' type, MT tiles of 8 rows of a, NT of 8 rows of W (with silu every other one of the up half), W waves, U blocks of 32 numbers of
-// k that a lane asks for at once
-template <typename T, int MT, int NT, int W, int U>
+// k that a lane asks for at once; NORMS: takes part in norms (GemmArgs)
+template <typename T, int MT, int NT, int W, int U, bool NORMS>
 __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(MT * NT * kFp4Terms<T> == 16 ? 2 : 1))) void fp4_lines_kernel(GemmArgs a) {
   constexpr int SP = kFp4Terms<T>;
   const int lane = threadIdx.x % kWave, r = lane % 16, g = lane / 16;
@@ -168,23 +177,47 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(MT * 
         }
       }
   };
+  static_assert(!NORMS || (MT == 1 && W == 8 && std::is_same_v<T, bf16>), "norms are of up to 8 bf16 rows");
+  // partial sums of four rows, which are added up behind the products; a thread a word, the rows' halves in turn.  (a.sums: of no meaning)
+  f32x4 some = {0.f, 0.f, 0.f, 0.f};
+  if (first < end) fetch(first);
+  if constexpr (NORMS) some = *reinterpret_cast<const f32x4*>((a.parts ? a.parts : a.sums) + 4 * min((int)threadIdx.x, max(2 * a.n_parts - 1, 0)));
   if (first < end) {
-    fetch(first);
     for (int i = first; i + 1 < end; ++i) turn(i, std::false_type{});
     turn(end - 1, std::true_type{});
   }
 
   __shared__ f32x4 part[W][NT * MT][kWave];
+  __shared__ float wave_sums[W][8], tile_sums[NT][8];
+  if constexpr (NORMS) {
+    some = (int)threadIdx.x < 2 * a.n_parts ? some : f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = threadIdx.x + W * kWave; i < 2 * a.n_parts; i += W * kWave) some += *reinterpret_cast<const f32x4*>(a.parts + 4 * (size_t)i);
+#pragma unroll
+    for (int d = 2; d < kWave; d *= 2)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) some[e] += __shfl_xor(some[e], d);
+    if (lane < 2) *reinterpret_cast<f32x4*>(&wave_sums[wave][4 * lane]) = some;
+  }
 #pragma unroll
   for (int p = 0; p < NT; ++p)
 #pragma unroll
     for (int t = 0; t < MT; ++t) part[wave][p * MT + t][lane] = acc[p][t];
   __syncthreads();
+  float root = 1.f;
+  if constexpr (NORMS) {
+    if (a.parts) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) sum += wave_sums[w][r % 8];
+      root = 1.f / sqrtf(sum / (a.blocks * kFp4Block) + a.eps);
+    }
+  }
   // lane (r, g) of a tile's total: rows 4 g .. of W, row r of a; the quarters g < 2, r < 8 and g >= 2, r >= 8 are of two runs of k
   auto total = [&](int tile) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < W; ++w) v += part[w][tile][lane] + part[w][tile][lane ^ 40];
+    if constexpr (NORMS) v *= root;
     return v;
   };
   if (silu && !a.slices) {
@@ -195,6 +228,34 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(MT * 
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = silu_times(gate[i], up[i]);
       if (m < a.M && r < 8 && g < 2) put(a, m, row_of(p) + 4 * g, half, v);
+    }
+  } else if (NORMS && a.h) {
+    for (int p = wave; p < NT; p += W) {
+      const f32x4 v = total(p);
+      const int n = row_of(p) + 4 * g;
+      float squares = 0.f;
+      if (r < a.M && r < 8 && g < 2 && n < a.N) {
+        f32x4* o = reinterpret_cast<f32x4*>((float*)a.out + (size_t)r * a.ldo + n);
+        const f32x4 x = *o + v;
+        *o = x;
+        bf16x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float gamma = a.gamma32 ? ((const float*)a.gamma)[n + i] : (float)((const bf16*)a.gamma)[n + i];
+          y[i] = (bf16)(gamma * x[i]);
+          squares = fmaf(x[i], x[i], squares);
+        }
+        *reinterpret_cast<bf16x4*>(a.h + (size_t)r * a.ldh + n) = y;
+      }
+      squares += __shfl_xor(squares, 16);
+      if (lane < 8) tile_sums[p][lane] = squares;
+    }
+    __syncthreads();
+    if (threadIdx.x < 8) {
+      float sum = 0.f;
+#pragma unroll
+      for (int p = 0; p < NT; ++p) sum += tile_sums[p][threadIdx.x];
+      a.sums[(size_t)nt * 8 + threadIdx.x] = sum;
     }
   } else {
     for (int u = wave; u < NT * MT; u += W) {
@@ -356,6 +417,7 @@ struct Form {
   float alone[2], busy[2];           // us of a turn with little and with much on the chip (bf16 rows, 32-bit ones), 0: not for such rows
 };
 static constexpr int kLinesForms = 5;
+static constexpr int kNormRows = 8;   // up to which a product takes part in norms (forms 0 to 2 with k whole)
 static constexpr Form kForms[] = {{32, 8, 64, {0.f, 0.f}, {1.9f, 3.1f}},         // lines: MT x NT 1 x 4, 8 waves
                                   {16, 8, 64, {0.f, 0.f}, {1.35f, 2.3f}},        // 1 x 2, 8
                                   {8, 8, 128, {0.f, 0.f}, {1.7f, 3.7f}},         // 1 x 1, 8 (U 2)
@@ -382,7 +444,7 @@ static Plan plan(int M, int N, int K, bool silu, int dtype, int most_slices) {
   };
   // up to 8 rows: as many rows of W a workgroup as leave about 192 of them (16 with silu, which takes pairs of tiles).  us, 8 rows: 6,144 of
   // 4,096 by 32 7.8, by 16 8.5; 2,560 of 2,560 by 16 5.3, by 8 6.1; 2,048 of 8,192 by 8 8.1, by 16 11.
-  if (M <= 8) return laid_out(N >= 6144 ? 0 : N >= 2560 || silu ? 1 : 2, 1);
+  if (M <= kNormRows) return laid_out(N >= 6144 ? 0 : N >= 2560 || silu ? 1 : 2, 1);
   // more: the form with the least time by a model, whose numbers are fitted to 21 products of 9 to 1,024 rows in every form, with weights from
   // memory (8 % off; its choice is 1 to 2 % slower than the best).  A product costs its launch, W's bytes at 11 TB/s, and its turns, one after
   // another, each as long as its own latency or as what the workgroups of a compute unit need together (lines: the blocks that the waves
@@ -413,7 +475,14 @@ static Plan plan(int M, int N, int K, bool silu, int dtype, int most_slices) {
 
 template <typename T, int MT, int NT, int W, int U> static void lines(const Plan& p, const GemmArgs& a, hipStream_t stream) {
   static_assert(MT * NT * W <= 64, "the waves' sums fill LDS");
-  hipLaunchKernelGGL((fp4_lines_kernel<T, MT, NT, W, U>), dim3((unsigned)((p.n_tiles + 7) / 8 * 8 * p.m_tiles), (unsigned)p.slices), dim3(W * kWave), 0, stream, a);
+  const dim3 grid((unsigned)((p.n_tiles + 7) / 8 * 8 * p.m_tiles), (unsigned)p.slices);
+  if constexpr (MT == 1 && std::is_same_v<T, bf16>) {
+    if (a.parts || a.h) {
+      hipLaunchKernelGGL((fp4_lines_kernel<T, MT, NT, W, U, true>), grid, dim3(W * kWave), 0, stream, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((fp4_lines_kernel<T, MT, NT, W, U, false>), grid, dim3(W * kWave), 0, stream, a);
 }
 template <typename T, int MT, int NT, int B> static void tiles(const Plan& p, const GemmArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL((fp4_tiles_kernel<T, MT, NT, B>), dim3((unsigned)((p.n_tiles + 7) / 8 * 8 * p.m_tiles), (unsigned)p.slices), dim3(256), 0, stream, a);
@@ -454,8 +523,15 @@ extern "C" long long gb_fp4_gemm_floats(int M, int N, int K, int epilogue, int d
   return p.slices > 1 ? (long long)p.slices * M * N : 0;
 }
 
-extern "C" int gb_fp4_gemm(const void* x, int dtype, int ldx, const void* codes, const void* scales, int scale_stride, void* out, int out_dtype,
-                           int ldo, int M, int N, int K, int epilogue, float* workspace, long long workspace_floats, hipStream_t stream) {
+// tiles whose sums of squares a product that adds up to 8 rows leaves for the norm behind it; 0: it does not
+extern "C" int gb_fp4_gemm_emit_parts(int M, int N) {
+  return M > 0 && M <= kNormRows && N > 0 && N % 8 == 0 ? plan(M, N, 32, false, kBF16, 1).n_tiles : 0;
+}
+
+// with what a product does for norms (GemmArgs)
+extern "C" int gb_fp4_gemm_norms(const void* x, int dtype, int ldx, const void* codes, const void* scales, int scale_stride, void* out, int out_dtype,
+                                 int ldo, int M, int N, int K, int epilogue, float* workspace, long long workspace_floats, const void* gamma,
+                                 int gamma_dtype, void* h, int ldh, float* sums, const float* parts, int n_parts, float eps, hipStream_t stream) {
   GB_REQUIRE(M >= 0 && N > 0 && K > 0 && K % 32 == 0, "fp4_gemm: bad sizes M=%d N=%d K=%d", M, N, K);
   GB_REQUIRE(epilogue >= 0 && epilogue <= 2 && (epilogue != 2 || N % 2 == 0), "fp4_gemm: epilogue %d of %d columns", epilogue, N);
   GB_REQUIRE(epilogue != 1 || out_dtype == kF32, "fp4_gemm: accumulation is into a 32-bit result");
@@ -463,17 +539,29 @@ extern "C" int gb_fp4_gemm(const void* x, int dtype, int ldx, const void* codes,
   GB_REQUIRE(scale_stride >= K / 32 && scale_stride % 16 == 0 && ((uintptr_t)codes & 15) == 0 && ((uintptr_t)scales & 15) == 0,
              "fp4_gemm: codes and scales begin at 16-byte words, rows of scales are multiples of 16");
   GB_REQUIRE((dtype == kF32 || dtype == kBF16) && (out_dtype == kF32 || out_dtype == kBF16), "fp4_gemm: unknown dtype %d or %d", dtype, out_dtype);
+  GB_REQUIRE(!h || (dtype == kBF16 && epilogue == 1 && M <= kNormRows && N % 8 == 0 && (uintptr_t)out % 16 == 0 && ldo % 4 == 0 && (uintptr_t)h % 8 == 0 &&
+                    ldh % 4 == 0 && ldh >= N && sums && gamma && (gamma_dtype == kF32 || gamma_dtype == kBF16)),
+             "fp4_gemm: a norm is prepared by products that add up to %d bfloat16 rows, of a multiple of 8 columns in whole words", kNormRows);
+  GB_REQUIRE(!parts || (dtype == kBF16 && epilogue != 1 && M <= kNormRows && n_parts > 0 && n_parts < (1 << 24) && (uintptr_t)parts % 16 == 0), "fp4_gemm: a norm's sums go with up to %d bfloat16 rows", kNormRows);
   if (M == 0) return 0;
   Plan p = plan(M, N, K, epilogue == 2, dtype, 16);
   if (p.slices > 1 && (!workspace || workspace_floats < (long long)p.slices * M * N)) p = plan(M, N, K, epilogue == 2, dtype, 1);   // slower, not refused
   GB_REQUIRE((long long)(p.n_tiles + 7) * p.m_tiles < (1ll << 31) && (long long)M * N < (1ll << 38), "fp4_gemm: %d x %d is too much for one launch", M, N);
   const int e = out_dtype == kF32 ? 16 : 8;   // bytes of four columns
-  const GemmArgs a{x, (const uint8_t*)codes, (const uint8_t*)scales, out, p.slices > 1 ? workspace : nullptr, ldx, ldo, M, N, K / 32, scale_stride,
+  const GemmArgs a{x, (const uint8_t*)codes, (const uint8_t*)scales, out, p.slices > 1 ? workspace : nullptr, parts, gamma,
+                   (bf16*)h, sums, n_parts, gamma_dtype == kF32, ldh, eps, ldx, ldo, M, N, K / 32, scale_stride,
                    p.n_tiles, p.m_tiles, p.turns, epilogue, out_dtype == kF32, (uintptr_t)out % e == 0 && ldo % 4 == 0};
   if (dtype == kF32) launch_by<float>(p, a, stream);
   else launch_by<bf16>(p, a, stream);
   return launched("fp4_gemm");
 }
 
+extern "C" int gb_fp4_gemm(const void* x, int dtype, int ldx, const void* codes, const void* scales, int scale_stride, void* out, int out_dtype,
+                           int ldo, int M, int N, int K, int epilogue, float* workspace, long long workspace_floats, hipStream_t stream) {
+  return gb_fp4_gemm_norms(x, dtype, ldx, codes, scales, scale_stride, out, out_dtype, ldo, M, N, K, epilogue, workspace, workspace_floats, nullptr, kF32,
+                           nullptr, 0, nullptr, nullptr, 0, 0.f, stream);
+}
+
 GB_TAPED(gb_fp4_gemm)
+GB_TAPED(gb_fp4_gemm_norms)
 GB_DEFINE_LAST_ERROR

@@ -290,8 +290,11 @@ _SIGS = {
         "gb_fp4_attention_floats": [_i, _i, _i, _i, _i, _i, _i, _i],
     },
     "fp4_gemm": {
-        # a, dtype, lda, codes, scales, scales a row, out, its dtype, ldo, M, N, K, epilogue, workspace, its floats, stream
+        # a, dtype, lda, codes, scales, scales a row, out, its dtype, ldo, M, N, K, epilogue, workspace, its floats, (gamma, its dtype, h, ldh,
+        # sums, parts, their number, eps,) stream
         "gb_fp4_gemm": [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, C.c_longlong, _vp],
+        "gb_fp4_gemm_norms": [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, C.c_longlong, _vp, _i, _vp, _i, _vp, _vp, _i, _f, _vp],
+        "gb_fp4_gemm_emit_parts": [_i, _i],
         "gb_fp4_gemm_floats": [_i, _i, _i, _i, _i],
     },
     "sampling": {
@@ -2820,11 +2823,21 @@ def fp4_gemm_floats(rows: int, n: int, k: int, dtype: torch.dtype = torch.bfloat
     return int(f(int(rows), int(n), int(k), 2 if silu_mul else 0, F32 if dtype == torch.float32 else BF16))
 
 
+@functools.lru_cache(maxsize=4096)   # a pure function of the sizes, asked for at every product
+def fp4_gemm_emit_parts(rows: int, n: int) -> int:
+    """How many partial sums an accumulating product of ``rows`` bfloat16 rows and ``n`` rows of w writes when asked to prepare the norm that
+    follows (``fp4_gemm(..., emit=...)``); 0 if it cannot."""
+    return int(_lib("fp4_gemm").gb_fp4_gemm_emit_parts(int(rows), int(n)))
+
+
 def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool = False, silu_mul: bool = False,
-             workspace: Optional[torch.Tensor] = None) -> None:
+             workspace: Optional[torch.Tensor] = None, emit: Optional[tuple] = None, rms_parts: Optional[tuple] = None) -> None:
     """out (+)= a . w^T with four-bit weights, the sums in 32 bits: ``a`` [rows, columns of w] bfloat16 or float32, ``out`` bfloat16 or float32
     (float32 when accumulating).  ``silu_mul``: w stacks gate rows over up rows and out[m, j] = silu(a . gate_j) * (a . up_j), of half as
     many columns.
+    ``emit=(gamma, h, parts)`` (accumulating, bfloat16 rows, where ``fp4_gemm_emit_parts`` is not 0): besides the new residual r in out,
+    h[m, n] = bf16(gamma[n] r[m, n]) and float32 parts[tile, m] of sum(r^2) over the tile's columns are written (``parts_stride(M)`` floats a tile), as
+    ``gemm`` does.  ``rms_parts=(parts, n_parts, eps)`` (up to 8 rows): a is such an h, and the product is scaled to that of the normed rows.
     ``workspace`` (float32, ``fp4_gemm_floats`` elements; optional): lets few workgroups divide k (their sums are added in a fixed order), and
     large bfloat16 products have the weights' bfloat16 values written there first and multiplied by ``gemm``."""
     N, K, each, c_at, s_at = _fp4_matrix(w, "fp4_gemm")
@@ -2840,6 +2853,9 @@ def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool 
     if M and not _apart(at, M, K * e, lda * e, to, M, (N // 2 if silu_mul else N) * f, ldo * f):
         raise KernelError("fp4_gemm: a and out share memory")
     ws_at, floats = _fp4_workspace(workspace, "fp4_gemm")
+    epilogue = 2 if silu_mul else 1 if accumulate else 0
+    if emit is not None or rms_parts is not None:
+        return _fp4_gemm_norms(a, w, out, (at, dtype, lda, c_at, s_at, each, to, out_dtype, ldo, M, N, K, epilogue, ws_at, floats), workspace, emit, rms_parts)
     here = _here("fp4_gemm", a, w[0], w[1], out, workspace)
     if floats >= N * K // 2 and _fp4_expands(M, N, K, a.dtype, out.dtype, silu_mul) and lda % 8 == 0 and at % 16 == 0:
         values, rest = workspace[:N * K // 2].view(torch.bfloat16).view(N, K), workspace[N * K // 2:]
@@ -2847,5 +2863,31 @@ def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool 
         gemm(a, values, out, accumulate=accumulate, silu_mul=silu_mul, workspace=rest if rest.numel() >= max(1, gemm_split_floats(M, N, K)) else None)
         return
     lib = _lib("fp4_gemm")
-    _launch(lib, lib.gb_fp4_gemm, at, dtype, lda, c_at, s_at, each, to, out_dtype, ldo, M, N, K,
-            2 if silu_mul else 1 if accumulate else 0, ws_at, floats, _stream_of(here))
+    _launch(lib, lib.gb_fp4_gemm, at, dtype, lda, c_at, s_at, each, to, out_dtype, ldo, M, N, K, epilogue, ws_at, floats, _stream_of(here))
+
+
+def _fp4_gemm_norms(a, w, out, args: tuple, workspace, emit: Optional[tuple], rms_parts: Optional[tuple]) -> None:
+    """``fp4_gemm`` with ``emit`` or ``rms_parts``: what is left to check, and the launch."""
+    dtype, M, N, accumulate = args[1], args[9], args[10], args[12] == 1
+    gamma = h = sums = parts = None
+    n_parts, eps, ldh = 0, 0.0, 0
+    if emit is not None:
+        gamma, h, sums = emit
+        if (not accumulate or dtype != BF16 or M > 8 or N % 8 or gamma.numel() != N or not gamma.is_contiguous() or h.dtype != torch.bfloat16
+                or h.shape != out.shape or sums.dtype is not _FLOAT or not sums.is_contiguous()):
+            raise KernelError("fp4_gemm: emit needs an accumulating product that fp4_gemm_emit_parts accepts, gamma of N entries, a bfloat16 [M, N] "
+                              "operand buffer and float32 parts")
+        ldh, at, lda, to, ldo = _rows(h, "emit h"), args[0], args[2], args[6], args[8]
+        if M and not (_apart(h.data_ptr(), M, 2 * N, 2 * ldh, at, M, 2 * args[11], 2 * lda) and _apart(h.data_ptr(), M, 2 * N, 2 * ldh, to, M, 4 * N, 4 * ldo)):
+            raise KernelError("fp4_gemm: the rows of emit share memory with a or out")
+    if rms_parts is not None:
+        parts, n_parts, eps = rms_parts
+        if (accumulate or dtype != BF16 or M > 8 or n_parts <= 0 or parts.dtype is not _FLOAT or not parts.is_contiguous() or parts.data_ptr() % 16
+                or parts.numel() < n_parts * parts_stride(M)):
+            raise KernelError("fp4_gemm: partial sums of a norm go with at most 8 bfloat16 rows and a storing product")
+    here = _here("fp4_gemm", a, w[0], w[1], out, workspace, gamma, h, sums, parts)
+    if sums is not None and sums.numel() < fp4_gemm_emit_parts(M, N) * parts_stride(M):
+        raise KernelError(f"fp4_gemm: emit needs parts_stride(M) float32 for each of {fp4_gemm_emit_parts(M, N)} parts, {sums.numel()} are given")
+    lib = _lib("fp4_gemm")
+    _launch(lib, lib.gb_fp4_gemm_norms, *args, _p(gamma), 0 if gamma is None else dtype_code(gamma), _p(h), ldh, _p(sums), _p(parts), n_parts, eps,
+            _stream_of(here))

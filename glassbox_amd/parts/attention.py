@@ -196,19 +196,19 @@ class PagedAttention(Mixer):
         return handed_on
 
     def _forward_fp4(self, ctx, h, residual, cache: LayerCache, norm, emit):
-        """``forward`` with matrices or pages, or both, of four-bit numbers: the norm (where the product does not take it), the
+        """``forward`` with matrices or pages, or both, of four-bit numbers: the norm (where no product does its work), the
         product, rotation and cache write, attention and the output projection are a launch each."""
         n = h.shape[0]
         rows = self.q_dim + (0 if self.shares_kv else 2 * self.kv_dim)
         n_kv = 0 if self.shares_kv else self.n_kv_heads
         qkv = ctx.buffer("qkv", (n, rows), ctx.dtype)
         packed, pre = self.wqkv_scales is not None, isinstance(norm, PreNormed)
-        if norm is not None and not pre and (packed or ctx.dtype == torch.float32):
+        if norm is not None and not packed and ctx.dtype == torch.float32:
             normed = ctx.buffer("h", (n, self.width), ctx.dtype)
             ops.rmsnorm(h, norm[0], norm[1], normed)
             h, norm = normed, None
-        if packed:   # (never with ``pre``: the matrices before this one are packed too, and their products prepare no norm)
-            fp4_product(ctx, h, self.wqkv, self.wqkv_scales, qkv)
+        if packed:
+            fp4_product(ctx, h, self.wqkv, self.wqkv_scales, qkv, norm=norm)
         elif pre:
             ops.gemm(norm.rows, self.wqkv, qkv, rms_parts=norm.as_gemm_arg())
         else:
@@ -227,8 +227,7 @@ class PagedAttention(Mixer):
             self.position.apply_and_store(ctx, qkv, self.n_heads, n_kv, self.head_dim, *store)
             paged_attention(ctx, qkv[:, :self.q_dim], att, cache, self.n_heads, self.scale, self.window)
         if packed:
-            fp4_product(ctx, att, self.wo, self.wo_scales, residual, accumulate=True)
-            return None
+            return fp4_product(ctx, att, self.wo, self.wo_scales, residual, accumulate=True, emit=emit, tag="mixer")
         target, handed_on = emit_target(ctx, n, self.width, self.q_dim, emit, "mixer")
         ops.gemm(att, self.wo, residual, accumulate=True, emit=target, workspace=split_workspace(ctx, n, self.width, self.q_dim))
         return handed_on

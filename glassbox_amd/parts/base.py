@@ -179,12 +179,27 @@ def needs_multiple_of_32(what: str, size: int) -> List[str]:
     return [f"{what}: {size} is not a multiple of 32, the block of a four-bit matrix"] if size % 32 else []
 
 
-def fp4_product(ctx, a, codes, scales, out, accumulate: bool = False, silu_mul: bool = False) -> None:
-    """``ops.fp4_gemm`` with the workspace that it has a use for in this step."""
+def fp4_product(ctx, a, codes, scales, out, accumulate: bool = False, silu_mul: bool = False, norm=None, emit=None, tag: str = ""):
+    """``ops.fp4_gemm`` with the workspace that it has a use for in this step.  ``norm``: a is the residual before this norm, ``(gamma, eps)``,
+    or what a product before it prepared of it (``PreNormed``).  ``emit=(gamma, eps)``: the product, which adds into the residual, may prepare
+    the norm that reads it next; returns a PreNormed if it did."""
     from .. import ops
-    floats = ops.fp4_gemm_floats(a.shape[0], codes.shape[0], a.shape[1], a.dtype, out.dtype, silu_mul)
-    ops.fp4_gemm(a, ops.Fp4Matrix(codes, scales), out, accumulate=accumulate, silu_mul=silu_mul,
-                 workspace=ctx.buffer("fp4_gemm", (floats,), torch.float32) if floats else None)
+    n, w, more, handed_on = a.shape[0], ops.Fp4Matrix(codes, scales), {}, None
+    if isinstance(norm, PreNormed):
+        a, more["rms_parts"] = norm.rows, norm.as_gemm_arg()
+    elif norm is not None:
+        a, x = ctx.buffer("h", tuple(a.shape), ctx.dtype), a
+        ops.rmsnorm(x, norm[0], norm[1], a)
+    if emit is not None and ctx.fuse_norms and a.dtype == torch.bfloat16:
+        n_parts = ops.fp4_gemm_emit_parts(n, codes.shape[0])
+        if n_parts:
+            rows = ctx.buffer(f"prenorm_rows_{tag}", tuple(out.shape), torch.bfloat16)
+            parts = ctx.buffer(f"prenorm_parts_{tag}", (n_parts, ops.parts_stride(n)), torch.float32)
+            more["emit"], handed_on = (emit[0], rows, parts), PreNormed(rows, parts, n_parts, float(emit[1]))
+    floats = ops.fp4_gemm_floats(n, codes.shape[0], a.shape[1], a.dtype, out.dtype, silu_mul)
+    ops.fp4_gemm(a, w, out, accumulate=accumulate, silu_mul=silu_mul, workspace=ctx.buffer("fp4_gemm", (floats,), torch.float32) if floats else None,
+                 **more)
+    return handed_on
 
 
 def needs_multiple_of_8(dtype: torch.dtype, what: str, size: int) -> List[Tuple[str, str]]:

@@ -61,14 +61,9 @@ class SwiGLU(FeedForward):
         ``store``: the rows are written to ``residual`` (float32) instead of added."""
         n = h.shape[0]
         act = ctx.buffer("act", (n, self.intermediate), ctx.dtype)
-        if self.w_gate_up_scales is not None:   # (no PreNormed: the mixer's matrices are packed too, and their products prepare no norm)
-            if norm is not None:
-                normed = ctx.buffer("h", (n, self.width), ctx.dtype)
-                ops.rmsnorm(h, norm[0], norm[1], normed)
-                h = normed
-            fp4_product(ctx, h, self.w_gate_up, self.w_gate_up_scales, act, silu_mul=True)
-            fp4_product(ctx, act, self.w_down, self.w_down_scales, residual, accumulate=not store)
-            return None
+        if self.w_gate_up_scales is not None:
+            fp4_product(ctx, h, self.w_gate_up, self.w_gate_up_scales, act, silu_mul=True, norm=norm)
+            return fp4_product(ctx, act, self.w_down, self.w_down_scales, residual, accumulate=not store, emit=None if store else emit, tag="ffn")
         if ctx.dtype == torch.bfloat16 and (self.width % 8 or self.intermediate % 8):
             # (only with ``any_size``, and then without norms to fuse: the blocks that offer those build it without)
             gate_up = ctx.buffer("gate_up", (n, 2 * self.intermediate), ctx.dtype)

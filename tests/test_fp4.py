@@ -36,12 +36,16 @@ def attention(**change):
 
 def gemm(**change):
     a = dict(a=torch.zeros(3, 64, dtype=BF), w=ops.Fp4Matrix(torch.zeros(10, 32, dtype=U8), torch.zeros(10, 16, dtype=U8)),
-             out=torch.zeros(3, 10, dtype=BF), accumulate=False, silu_mul=False)
+             out=torch.zeros(3, 10, dtype=BF), accumulate=False, silu_mul=False,
+             emit=None, rms_parts=None)
     a.update(change)
-    ops.fp4_gemm(a["a"], a["w"], a["out"], accumulate=a["accumulate"], silu_mul=a["silu_mul"])
+    ops.fp4_gemm(a["a"], a["w"], a["out"], accumulate=a["accumulate"], silu_mul=a["silu_mul"], emit=a["emit"], rms_parts=a["rms_parts"])
 
 
 ROWS = torch.zeros(5, 512, dtype=BF)
+ADDS = dict(out=torch.zeros(3, 10), accumulate=True)
+ADDS8 = dict(out=torch.zeros(3, 16), accumulate=True, w=ops.Fp4Matrix(torch.zeros(16, 32, dtype=U8), torch.zeros(16, 16, dtype=U8)))
+EMIT = (torch.ones(16), torch.zeros(3, 16, dtype=BF), torch.zeros(8, 8))
 REFUSED = [
     (store, dict(D=48), "multiple of 32"), (store, dict(G=3), "do not hold"), (store, dict(qkv=torch.zeros(5, 511, dtype=BF)), "do not hold"),
     (store, dict(k=pages(d=128)), "alike"), (store, dict(k=pages(g=1), v=pages(g=1)), "kv heads"), (store, dict(k=pages().view(torch.int8)), "uint8"),
@@ -71,6 +75,16 @@ REFUSED = [
     (gemm, dict(w=ops.Fp4Matrix(torch.zeros(0, 32, dtype=U8), torch.zeros(0, 16, dtype=U8)), out=torch.zeros(3, 0, dtype=BF)), "four-bit matrix"),
     (gemm, dict(a=torch.zeros(3, 64, dtype=torch.float16)), "element type"), (gemm, dict(a=torch.zeros(64, 3, dtype=BF).t()), "dense rows"),
     (gemm, dict(a=ROWS[:3, :64], out=ROWS[:3, 60:70]), "share memory"), (gemm, {}, "current GPU"),
+    (gemm, dict(ADDS, emit=(torch.ones(10), torch.zeros(3, 10, dtype=BF), torch.zeros(8, 8))), "emit needs"),           # 10 columns
+    (gemm, dict(ADDS8, accumulate=False, emit=EMIT), "emit needs"), (gemm, dict(ADDS8, a=torch.zeros(3, 64), emit=EMIT), "emit needs"),
+    (gemm, dict(ADDS8, emit=(torch.ones(15), *EMIT[1:])), "emit needs"), (gemm, dict(ADDS8, emit=(EMIT[0], torch.zeros(3, 16), EMIT[2])), "emit needs"),
+    (gemm, dict(ADDS8, emit=(*EMIT[:2], torch.zeros(8, 8, dtype=BF))), "emit needs"), (gemm, dict(ADDS8, emit=EMIT), "current GPU"),
+    (gemm, dict(ADDS8, a=torch.zeros(9, 64, dtype=BF), out=torch.zeros(9, 16), emit=(EMIT[0], torch.zeros(9, 16, dtype=BF), torch.zeros(8, 64))), "emit needs"),
+    (gemm, dict(ADDS8, a=ROWS[:3, :64], emit=(EMIT[0], ROWS[:3, 60:76], EMIT[2])), "share memory"),
+    (gemm, dict(rms_parts=(torch.zeros(2, 8), 3, 1e-5)), "partial sums"), (gemm, dict(rms_parts=(torch.zeros(17)[1:].view(2, 8), 2, 1e-5)), "partial sums"), (gemm, dict(rms_parts=(torch.zeros(2, 8), 0, 1e-5)), "partial sums"),
+    (gemm, dict(ADDS8, rms_parts=(torch.zeros(2, 8), 2, 1e-5)), "partial sums"), (gemm, dict(a=torch.zeros(3, 64), rms_parts=(torch.zeros(2, 8), 2, 1e-5)), "partial"),
+    (gemm, dict(a=torch.zeros(9, 64, dtype=BF), out=torch.zeros(9, 10, dtype=BF), rms_parts=(torch.zeros(2, 64), 2, 1e-5)), "partial sums"),
+    (gemm, dict(rms_parts=(torch.zeros(2, 8), 2, 1e-5)), "current GPU"),
     (lambda **k: ops.fp4_quantize(**k), dict(w=torch.zeros(4, 40)), "multiple of 32"), (lambda **k: ops.fp4_quantize(**k), dict(w=torch.zeros(4, 0)), "multiple"),
     (lambda **k: ops.fp4_quantize(**k), dict(w=torch.zeros(4, 32, dtype=torch.float16)), "element type"),
     (lambda **k: ops.fp4_quantize(**k), dict(w=torch.zeros(4, 32)), "current GPU"),

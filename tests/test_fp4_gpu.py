@@ -572,3 +572,45 @@ def test_gemm_through_the_values_into_rows_that_begin_anywhere(how):
         assert not odd or ((out[:, :odd] == 2).all() and (out[:, odd + cols:] == 2).all())
         outs.append(out[:, odd:odd + cols])
     assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 64, 96), (8, 2048, 544), (3, 2592, 160), (7, 6176, 64), (5, 40, 32), (8, 4096, 4128), (2, 4128, 64)])
+@pytest.mark.parametrize("gamma_dtype", [torch.float32, torch.bfloat16])
+def test_a_product_prepares_a_norm_and_the_next_takes_it(M, N, K, gamma_dtype):
+    from glassbox_amd import ops
+    w = ops.fp4_quantize(normal(N, K, seed=60, scale=0.05).to(DEV))
+    wd = torch.empty(N, K, device=DEV)
+    ops.fp4_expand(w, wd)
+    a, first = normal(M, K, seed=61, wide=4.0).bfloat16().to(DEV), normal(M, N, seed=62, wide=3.0).to(DEV)
+    gamma = (normal(N, seed=63) + 1).to(gamma_dtype).to(DEV)
+    tiles, eps = ops.fp4_gemm_emit_parts(M, N), 1e-5
+    assert tiles > 0
+    x, plain_x = first.clone(), first.clone()
+    h = torch.full((M, N + 8), 3.0, dtype=torch.bfloat16, device=DEV)
+    parts = torch.full((tiles + 1, ops.parts_stride(M)), 7.0, device=DEV)
+    ops.fp4_gemm(a, w, x, accumulate=True, emit=(gamma, h[:, :N], parts))
+    ops.fp4_gemm(a, w, plain_x, accumulate=True)
+    assert torch.equal(x, plain_x)                                   # the residual is what it is without
+    assert torch.equal(h[:, :N], (gamma.float() * x).bfloat16()) and (h[:, N:] == 3).all() and (parts[tiles:] == 7).all()
+    with pytest.raises(ops.KernelError, match="each of"):
+        ops.fp4_gemm(a, w, plain_x, accumulate=True, emit=(gamma, h[:, :N], parts.flatten()[:tiles * 8 - 1]))
+    squares = (x.double() ** 2).sum(-1)
+    assert ((parts[:tiles, :M].double().sum(0) - squares).abs() <= (N / 2 + 8) * STEP * squares).all()   # (half a step for each addition)
+    if N % 32:
+        return
+    w2 = ops.fp4_quantize(normal(98, N, seed=64, scale=0.05).to(DEV))
+    wd2 = torch.empty(98, N, device=DEV)
+    ops.fp4_expand(w2, wd2)
+    root = 1 / torch.sqrt(squares / N + eps)
+    rows = h[:, :N].double()
+    y, size = rows @ wd2.double().t() * root[:, None], rows.abs() @ wd2.double().abs().t() * root[:, None]
+    off = (3 * N + 16 + N / 2 + 16) * STEP * size                    # the sums; the root of a sum of N squares and of as many partial sums
+    for out_dtype in (torch.bfloat16, torch.float32):
+        out = torch.empty(M, 98, dtype=out_dtype, device=DEV)
+        ops.fp4_gemm(h[:, :N], w2, out, rms_parts=(parts, tiles, eps))
+        assert ((out.double() - y).abs() <= off + half_step(out_dtype) * (y.abs() + off)).all()
+        out = torch.empty(M, 49, dtype=out_dtype, device=DEV)
+        ops.fp4_gemm(h[:, :N], w2, out, silu_mul=True, rms_parts=(parts, tiles, eps))
+        g, u, dg, du = y[:, :49], y[:, 49:], off[:, :49], off[:, 49:]
+        z, dz = g * torch.sigmoid(g) * u, 1.1 * dg * (u.abs() + du) + (g.abs() + dg) * du + 8 * STEP * (g * u).abs()
+        assert ((out.double() - z).abs() <= dz + half_step(out_dtype) * (z.abs() + dz) + 1e-30).all()
