@@ -177,11 +177,15 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(MT * 
         }
       }
   };
-  static_assert(!NORMS || (MT == 1 && W == 8 && std::is_same_v<T, bf16>), "norms are of up to 8 bf16 rows");
-  // partial sums of four rows, which are added up behind the products; a thread a word, the rows' halves in turn.  (a.sums: of no meaning)
-  f32x4 some = {0.f, 0.f, 0.f, 0.f};
+  static_assert(!NORMS || (MT == 1 && std::is_same_v<T, bf16>), "norms are of up to 8 bf16 rows");
+  // partial sums of four rows, which are added up behind the products; a word in turn, the rows' halves in turn.  (a.sums: of no meaning)
+  constexpr int kWords = 8 / W;   // a thread: 256 parts
+  f32x4 some[kWords];
   if (first < end) fetch(first);
-  if constexpr (NORMS) some = *reinterpret_cast<const f32x4*>((a.parts ? a.parts : a.sums) + 4 * min((int)threadIdx.x, max(2 * a.n_parts - 1, 0)));
+  if constexpr (NORMS)
+#pragma unroll
+    for (int k = 0; k < kWords; ++k)
+      some[k] = *reinterpret_cast<const f32x4*>((a.parts ? a.parts : a.sums) + 4 * min((int)threadIdx.x + k * W * kWave, max(2 * a.n_parts - 1, 0)));
   if (first < end) {
     for (int i = first; i + 1 < end; ++i) turn(i, std::false_type{});
     turn(end - 1, std::true_type{});
@@ -190,13 +194,16 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(MT * 
   __shared__ f32x4 part[W][NT * MT][kWave];
   __shared__ float wave_sums[W][8], tile_sums[NT][8];
   if constexpr (NORMS) {
-    some = (int)threadIdx.x < 2 * a.n_parts ? some : f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int i = threadIdx.x + W * kWave; i < 2 * a.n_parts; i += W * kWave) some += *reinterpret_cast<const f32x4*>(a.parts + 4 * (size_t)i);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kWords; ++k)
+      if ((int)threadIdx.x + k * W * kWave < 2 * a.n_parts) sum += some[k];
+    for (int i = threadIdx.x + kWords * W * kWave; i < 2 * a.n_parts; i += W * kWave) sum += *reinterpret_cast<const f32x4*>(a.parts + 4 * (size_t)i);
 #pragma unroll
     for (int d = 2; d < kWave; d *= 2)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) some[e] += __shfl_xor(some[e], d);
-    if (lane < 2) *reinterpret_cast<f32x4*>(&wave_sums[wave][4 * lane]) = some;
+      for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], d);
+    if (lane < 2) *reinterpret_cast<f32x4*>(&wave_sums[wave][4 * lane]) = sum;
   }
 #pragma unroll
   for (int p = 0; p < NT; ++p)
@@ -416,13 +423,15 @@ struct Form {
   int rows_w, rows_a, step;          // a workgroup's rows of W and of a, blocks of k a turn
   float alone[2], busy[2];           // us of a turn with little and with much on the chip (bf16 rows, 32-bit ones), 0: not for such rows
 };
-static constexpr int kLinesForms = 5;
-static constexpr int kNormRows = 8;   // up to which a product takes part in norms (forms 0 to 2 with k whole)
+static constexpr int kLinesForms = 7;
+static constexpr int kNormRows = 8;   // up to which a product takes part in norms (lines, with k whole)
 static constexpr Form kForms[] = {{32, 8, 64, {0.f, 0.f}, {1.9f, 3.1f}},         // lines: MT x NT 1 x 4, 8 waves
                                   {16, 8, 64, {0.f, 0.f}, {1.35f, 2.3f}},        // 1 x 2, 8
                                   {8, 8, 128, {0.f, 0.f}, {1.7f, 3.7f}},         // 1 x 1, 8 (U 2)
                                   {64, 16, 32, {0.f, 0.f}, {2.3f, 4.9f}},        // 2 x 8, 4
                                   {32, 16, 64, {0.f, 0.f}, {2.9f, 5.5f}},        // 2 x 4, 8
+                                  {32, 8, 32, {0.f, 0.f}, {0.f, 0.f}},           // 1 x 4, 4 (not beyond 8 rows)
+                                  {64, 8, 32, {0.f, 0.f}, {0.f, 0.f}},           // 1 x 8, 4 (nor this)
                                   {64, 32, 8, {0.95f, 0.f}, {0.6f, 0.f}},        // tiles: 2 x 1, 8 blocks
                                   {128, 32, 8, {1.4f, 0.f}, {1.05f, 0.f}},       // 2 x 2, 8
                                   {128, 64, 8, {2.f, 0.f}, {1.4f, 0.f}},         // 4 x 2, 8
@@ -444,7 +453,14 @@ static Plan plan(int M, int N, int K, bool silu, int dtype, int most_slices) {
   };
   // up to 8 rows: as many rows of W a workgroup as leave about 192 of them (16 with silu, which takes pairs of tiles).  us, 8 rows: 6,144 of
   // 4,096 by 32 7.8, by 16 8.5; 2,560 of 2,560 by 16 5.3, by 8 6.1; 2,048 of 8,192 by 8 8.1, by 16 11.
-  if (M <= kNormRows) return laid_out(N >= 6144 ? 0 : N >= 2560 || silu ? 1 : 2, 1);
+  // Many rows of W: workgroups of four waves, which take more turns each: 1 row by 128,256 of 4,096 62, in eight waves 66; by 49,152 of 2,048 13.7 and
+  // 16.8.  With more rows of a, and 32-bit ones, by 64 rows of W, sooner where k is long: 4 rows by 128,256 of 4,096 61, by 32 69, in eight waves 70;
+  // 4 by 49,152 of 2,048 16.8, by 32 15.8; 8 by 28,672 of 4,096 21.6, by 32 24.0, in eight waves 24.2; 8 32-bit ones 27.8 and, in eight waves, 35.3.
+  if (M <= kNormRows) {
+    if (N >= 16384 && M <= (K >= 4096 ? 2 : 4) && dtype == kBF16) return laid_out(5, 1);
+    if (N >= 24576 || (N >= 16384 && M > 4)) return laid_out(6, 1);
+    return laid_out(N >= 6144 ? 0 : N >= 2560 || silu ? 1 : 2, 1);
+  }
   // more: the form with the least time by a model, whose numbers are fitted to 21 products of 9 to 1,024 rows in every form, with weights from
   // memory (8 % off; its choice is 1 to 2 % slower than the best).  A product costs its launch, W's bytes at 11 TB/s, and its turns, one after
   // another, each as long as its own latency or as what the workgroups of a compute unit need together (lines: the blocks that the waves
@@ -495,14 +511,16 @@ template <typename T> static void launch_by(const Plan& p, const GemmArgs& a, hi
     case 2: lines<T, 1, 1, 8, 2>(p, a, stream); break;
     case 3: lines<T, 2, 8, 4, 1>(p, a, stream); break;
     case 4: lines<T, 2, 4, 8, 1>(p, a, stream); break;
+    case 5: lines<T, 1, 4, 4, 1>(p, a, stream); break;
+    case 6: lines<T, 1, 8, 4, 1>(p, a, stream); break;
     default:
       if constexpr (std::is_same_v<T, float>) {
-        if (p.form == 9) tiles<T, 2, 1, 4>(p, a, stream);
+        if (p.form == 11) tiles<T, 2, 1, 4>(p, a, stream);
         else tiles<T, 2, 2, 4>(p, a, stream);
       } else {
-        if (p.form == 5) tiles<T, 2, 1, 8>(p, a, stream);
-        else if (p.form == 6) tiles<T, 2, 2, 8>(p, a, stream);
-        else if (p.form == 7) tiles<T, 4, 2, 8>(p, a, stream);
+        if (p.form == 7) tiles<T, 2, 1, 8>(p, a, stream);
+        else if (p.form == 8) tiles<T, 2, 2, 8>(p, a, stream);
+        else if (p.form == 9) tiles<T, 4, 2, 8>(p, a, stream);
         else tiles<T, 4, 4, 4>(p, a, stream);
       }
   }

@@ -333,6 +333,7 @@ GEMMS = [(1, 1, 32), (1, 40, 64), (3, 17, 96), (16, 64, 512), (17, 130, 544), (5
          (130, 1040, 256), (16, 17000, 96), (9, 520, 4128), (1, 8200, 1056), (2, 33000, 128), (20, 16500, 160), (300, 70, 992),
          # (each of the kernels' forms, with k whole and divided, one tile of rows and several)
          (9, 4100, 544), (9, 8200, 544), (17, 4100, 544), (9, 2050, 8224), (30, 1040, 8224), (17, 520, 8224), (9, 4100, 4128), (700, 70, 4128),
+         (8, 16400, 96), (5, 24600, 544), (3, 20000, 1056), (1, 25000, 2080),
          (33, 6150, 2080), (65, 12300, 96), (65, 6150, 4128), (33, 6150, 8224), (130, 1000, 960)]
 
 
@@ -574,7 +575,7 @@ def test_gemm_through_the_values_into_rows_that_begin_anywhere(how):
     assert torch.equal(outs[0], outs[1])
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 64, 96), (8, 2048, 544), (3, 2592, 160), (7, 6176, 64), (5, 40, 32), (8, 4096, 4128), (2, 4128, 64)])
+@pytest.mark.parametrize("M,N,K", [(1, 64, 96), (8, 2048, 544), (3, 2592, 160), (7, 6176, 64), (5, 40, 32), (8, 4096, 4128), (2, 4128, 64), (3, 16416, 32), (8, 16416, 32)])
 @pytest.mark.parametrize("gamma_dtype", [torch.float32, torch.bfloat16])
 def test_a_product_prepares_a_norm_and_the_next_takes_it(M, N, K, gamma_dtype):
     from glassbox_amd import ops
@@ -598,19 +599,20 @@ def test_a_product_prepares_a_norm_and_the_next_takes_it(M, N, K, gamma_dtype):
     assert ((parts[:tiles, :M].double().sum(0) - squares).abs() <= (N / 2 + 8) * STEP * squares).all()   # (half a step for each addition)
     if N % 32:
         return
-    w2 = ops.fp4_quantize(normal(98, N, seed=64, scale=0.05).to(DEV))
-    wd2 = torch.empty(98, N, device=DEV)
+    C = 98 if N > 2592 else 16402
+    w2 = ops.fp4_quantize(normal(C, N, seed=64, scale=0.05).to(DEV))
+    wd2 = torch.empty(C, N, device=DEV)
     ops.fp4_expand(w2, wd2)
     root = 1 / torch.sqrt(squares / N + eps)
     rows = h[:, :N].double()
     y, size = rows @ wd2.double().t() * root[:, None], rows.abs() @ wd2.double().abs().t() * root[:, None]
     off = (3 * N + 16 + N / 2 + 16) * STEP * size                    # the sums; the root of a sum of N squares and of as many partial sums
     for out_dtype in (torch.bfloat16, torch.float32):
-        out = torch.empty(M, 98, dtype=out_dtype, device=DEV)
+        out = torch.empty(M, C, dtype=out_dtype, device=DEV)
         ops.fp4_gemm(h[:, :N], w2, out, rms_parts=(parts, tiles, eps))
         assert ((out.double() - y).abs() <= off + half_step(out_dtype) * (y.abs() + off)).all()
-        out = torch.empty(M, 49, dtype=out_dtype, device=DEV)
+        out = torch.empty(M, C // 2, dtype=out_dtype, device=DEV)
         ops.fp4_gemm(h[:, :N], w2, out, silu_mul=True, rms_parts=(parts, tiles, eps))
-        g, u, dg, du = y[:, :49], y[:, 49:], off[:, :49], off[:, 49:]
+        g, u, dg, du = y[:, :C // 2], y[:, C // 2:], off[:, :C // 2], off[:, C // 2:]
         z, dz = g * torch.sigmoid(g) * u, 1.1 * dg * (u.abs() + du) + (g.abs() + dg) * du + 8 * STEP * (g * u).abs()
         assert ((out.double() - z).abs() <= dz + half_step(out_dtype) * (z.abs() + dz) + 1e-30).all()
