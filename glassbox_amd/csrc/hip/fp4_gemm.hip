@@ -9,14 +9,14 @@
 //   of W a tile, lanes r >= 8 with the same rows 128 numbers further on, so that a wave's load reads 8 whole lines of 128 bytes; the rows of
 //   a stand in the columns likewise, 8 of them, and of the 16 x 16 results the two quarters in which both are of one run of k are added up.
 //   The waves of a workgroup take turns over k and are joined through LDS.  (16 rows of W and half lines, us: 1 row by 128,256 of 4,096
-//   68.5, whole lines 55.8: 5.0 TB/s; 28,672 of 4,096 20.3 and 17.3; 2,048 of 8,192 7.1 and 5.4.)
+//   68.5, whole lines 62: 4.5 TB/s; 28,672 of 4,096 20.3 and 19; 2,048 of 8,192 7.1 and 5.4.)
 // tiles (more): a's rows go through LDS, 64 or 32 of them by 64 to 256 rows of W, whose waves have rows of W of their own: 2,048 rows by
 //   28,672 of 4,096 in 537 us, 0.9 PFLOP/s; 64 rows in 39.  (Rows of a from memory to every wave: 60; what bounds it there is the way into a
 //   compute unit, 20 to 50 GB/s each.)
-// Measured and left: workgroups that go on from tile to tile with the next one's lines under way (8 rows by 28,672 of 4,096 25.6, like this 22.7:
+// Measured and left: workgroups that go on from tile to tile with the next one's lines under way (8 rows by 28,672 of 4,096 25.6, like this 21.6:
 // more registers, fewer waves); an RMS norm of the rows on the way (41, and 25.5 with the norm in a launch of its own: rows of 32 bits and
 // gamma are three times the bytes into every compute unit).  What a norm costs up to 8 rows, where the product before prepares it (gamma x in bf16 and
-// partial sums of squares) and this one divides by the root: 8 rows by 4,096 of 4,096, then by 28,672 31.4 us for both, 32.9 with a launch between.
+// partial sums of squares) and this one divides by the root: 8 rows by 4,096 of 4,096, then by 28,672 27.6 us for both, 29.6 with a launch between.
 #include "fp4.h"
 
 #include <algorithm>
