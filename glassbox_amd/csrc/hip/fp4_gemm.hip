@@ -454,10 +454,11 @@ static Plan plan(int M, int N, int K, bool silu, int dtype, int most_slices) {
   // up to 8 rows: as many rows of W a workgroup as leave about 192 of them (16 with silu, which takes pairs of tiles).  us, 8 rows: 6,144 of
   // 4,096 by 32 7.8, by 16 8.5; 2,560 of 2,560 by 16 5.3, by 8 6.1; 2,048 of 8,192 by 8 8.1, by 16 11.
   // Many rows of W: workgroups of four waves, which take more turns each: 1 row by 128,256 of 4,096 62, in eight waves 66; by 49,152 of 2,048 13.7 and
-  // 16.8.  With more rows of a, and 32-bit ones, by 64 rows of W, sooner where k is long: 4 rows by 128,256 of 4,096 61, by 32 69, in eight waves 70;
-  // 4 by 49,152 of 2,048 16.8, by 32 15.8; 8 by 28,672 of 4,096 21.6, by 32 24.0, in eight waves 24.2; 8 32-bit ones 27.8 and, in eight waves, 35.3.
+  // 16.8.  With more rows of a, and 32-bit ones, by 64 rows of W: 4 rows by 128,256 of 4,096 61, by 32 69, in eight waves 70 (by 49,152 of 2,048
+  // 16.8, 15.8, 18.3); 8 by 28,672 of 4,096 21.6, by 32 24.0, in eight waves 24.2; 8 32-bit ones 27.8 and, in eight waves, 35.3.  k has no part in the
+  // choice: whoever takes a norm's partial sums asks for their number without it.
   if (M <= kNormRows) {
-    if (N >= 16384 && M <= (K >= 4096 ? 2 : 4) && dtype == kBF16) return laid_out(5, 1);
+    if (N >= 16384 && M <= (N < 24576 ? 4 : 2) && dtype == kBF16) return laid_out(5, 1);
     if (N >= 24576 || (N >= 16384 && M > 4)) return laid_out(6, 1);
     return laid_out(N >= 6144 ? 0 : N >= 2560 || silu ? 1 : 2, 1);
   }

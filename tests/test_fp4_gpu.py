@@ -575,7 +575,8 @@ def test_gemm_through_the_values_into_rows_that_begin_anywhere(how):
     assert torch.equal(outs[0], outs[1])
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 64, 96), (8, 2048, 544), (3, 2592, 160), (7, 6176, 64), (5, 40, 32), (8, 4096, 4128), (2, 4128, 64), (3, 16416, 32), (8, 16416, 32)])
+@pytest.mark.parametrize("M,N,K", [(1, 64, 96), (8, 2048, 544), (3, 2592, 160), (7, 6176, 64), (5, 40, 32), (8, 4096, 4128), (2, 4128, 64), (3, 16416, 32), (8, 16416, 32),
+                                   (4, 24608, 4128), (2, 24608, 4128)])
 @pytest.mark.parametrize("gamma_dtype", [torch.float32, torch.bfloat16])
 def test_a_product_prepares_a_norm_and_the_next_takes_it(M, N, K, gamma_dtype):
     from glassbox_amd import ops
