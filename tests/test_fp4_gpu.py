@@ -379,7 +379,7 @@ def test_gemm(M, N, K, dtype, out_dtype, how):
             assert (out[:, :odd] == 3).all() and (out[:, odd + cols:] == 3).all()
 
 
-@pytest.mark.parametrize("M,N,K,how", [(1540, 8208, 8192, "silu"), (1600, 8200, 8192, "add"), (1536, 2064, 2048, "silu"), (770, 4100, 4128, "store"), (700, 8300, 640, "store"), (260, 28672, 96, "silu")])
+@pytest.mark.parametrize("M,N,K,how", [(1540, 8208, 8192, "silu"), (1600, 8200, 8192, "add"), (1536, 2064, 2048, "silu"), (770, 4100, 4128, "store"), (1537, 2051, 2080, "store"), (771, 4099, 4128, "add"), (700, 8300, 640, "store"), (260, 28672, 96, "silu")])
 def test_gemm_of_many_rows(M, N, K, how):
     """Through the weights' values and in tiles, with the workspace and without it: of one size within rounding."""
     from glassbox_amd import ops
