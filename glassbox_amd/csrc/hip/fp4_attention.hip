@@ -129,7 +129,7 @@ __device__ __forceinline__ uint32_t mask_scores(f32x4 (&sc)[4], int key, bool kn
 
 // One step of the running softmax of a column (this lane's 16 keys of 64): probabilities as the product's operand, sums rescaled where
 // the maximum grows.  Their sum is a product with ones, of what the values are multiplied by and over all 64 (added up by the lanes: 2,048 rows of 32
-// heads of 128 62.6 us for 60.6, 131 rows behind 3,900 26.7 for 26.2).
+// heads of 128 62.6 us for 60.6, 131 rows behind 3,900 26.7 for 26.2, two tiles a wave).
 template <int SP, int NB>
 __device__ __forceinline__ void soften(const f32x4 (&sc)[4], float scale, float& m, f32x4& l, f32x4 (&o)[2 * NB], bf16x8 (&pf)[SP][2]) {
   float top = -__builtin_inff();
@@ -531,17 +531,18 @@ static Plan plan(int n_seqs, int nkv, int rep, int hd, int max_q, int max_contex
     if (max_context <= 1024) runs = 1;
     return laid_out(false, 1, runs, 512, 8 * kTile);
   }
-  // More: one tile of columns a wave or two (where they fit the registers), and as many runs, as take least by a model with numbers fitted to 1,900 launches
-  // (70 sizes, 9 % off; its choice is 2.5 % slower than the best, at most 18): a wave's turns, each `alone` us; the tiles that a SIMD has to do on
+  // More: one tile of columns a wave, two (where they fit the registers) or three (heads of 64: of 32 they gain nothing), and as many runs, as take least by a model with numbers fitted to some 2,000
+  // launches (70 sizes, 9 % off; its choice is 3 % slower than the best, at most 18): a wave's turns, each `alone` us; the tiles that a SIMD has to do on
   // average, `busy` us each, more where the workgroups do not divide evenly by the compute units; the joining of runs, its launch and its
-  // bytes.  us: 131 rows behind 3,900, 32 heads of 64 and as many kv heads, two tiles in 8 runs 28.4, in 5 31.9, one tile in 8 30.2; 8 kv heads of 128 two
-  // in 6 33.4, in 8 38.6; 1,024 rows of 32 heads of 64 two in one run 23, in two 43; 8 x 50 rows behind 550 one in one 16, two in three 25.
-  static constexpr float kAlone[2][9] = {{0.f, 0.4f, 0.55f, 1.2f, 0.75f, 0.f, 0.f, 0.f, 1.f}, {0.f, 0.55f, 0.65f, 1.35f, 1.05f}};   // by tiles and blocks a head
-  static constexpr float kBusy[2][9] = {{0.f, 0.55f, 0.65f, 1.1f, 0.83f, 0.f, 0.f, 0.f, 2.2f}, {0.f, 0.62f, 0.84f, 1.2f, 0.91f}};
+  // bytes.  us: 131 rows behind 3,900, 32 heads of 64 and as many kv heads, three tiles in 8 runs 24.3, two in 11 26.6, one in 8 30.2; 8 kv heads of 128 two
+  // in 6 33.4, in 8 38.6; 1,024 rows of 32 heads of 64 two in one run 23, in two 43; 8 x 50 rows behind 550 one in one 16, two in three 25;
+  // 131 rows behind 15,869, 32 heads of 64, three in 16 52, two in 10 59; 300 behind 15,700 91 and 104.
+  static constexpr float kAlone[3][9] = {{0.f, 0.38f, 0.48f, 1.2f, 0.75f, 0.f, 0.f, 0.f, 1.f}, {0.f, 0.55f, 0.59f, 1.35f, 1.01f}, {0.f, 0.f, 0.89f}};   // by tiles and blocks a head
+  static constexpr float kBusy[3][9] = {{0.f, 0.52f, 0.65f, 1.1f, 0.84f, 0.f, 0.f, 0.f, 2.2f}, {0.f, 0.59f, 0.8f, 1.2f, 0.91f}, {0.f, 0.f, 0.9f}};
   const bool wide = dtype == kF32;
   Plan best{};
   float least = 0.f;
-  for (int r = 1; r <= (!wide && hd <= 128 ? 2 : 1); ++r) {
+  for (int r = 1; r <= (wide || hd > 128 ? 1 : hd == 64 ? 3 : 2); ++r) {
     const float alone = kAlone[r - 1][hd / 32] * (wide ? 1.25f : 1.f), busy = kBusy[r - 1][hd / 32] * (wide ? 1.65f : 1.f);
     const float waves = (float)n_seqs * nkv * (float)((columns + 16 * r - 1) / (16 * r));
     for (int runs : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64}) {
@@ -562,7 +563,10 @@ template <typename T, int NB> static void launch(const Plan& p, const AttendArgs
   const dim3 grid((unsigned)((long long)n_seqs * a.nkv * p.col_tiles * p.splits));
   if (!p.cols) hipLaunchKernelGGL((fp4_attend_keys_kernel<T, NB, W>), grid, dim3(W * kWave), 0, stream, a);
   else if (p.r == 1) hipLaunchKernelGGL((fp4_attend_cols_kernel<T, NB, 1>), grid, dim3(4 * kWave), 0, stream, a);
-  else if constexpr (std::is_same_v<T, bf16> && NB <= 4) hipLaunchKernelGGL((fp4_attend_cols_kernel<T, NB, 2>), grid, dim3(4 * kWave), 0, stream, a);
+  else if constexpr (std::is_same_v<T, bf16> && NB <= 4) {
+    if (p.r == 2) hipLaunchKernelGGL((fp4_attend_cols_kernel<T, NB, 2>), grid, dim3(4 * kWave), 0, stream, a);
+    else if constexpr (NB == 2) hipLaunchKernelGGL((fp4_attend_cols_kernel<T, NB, 3>), grid, dim3(4 * kWave), 0, stream, a);
+  }
   if (p.splits > 1) {
     const int columns = n_seqs * a.nkv * a.max_q * a.rep;
     hipLaunchKernelGGL((fp4_join_kernel<T, NB * kFp4Block>), dim3((columns + 3) / 4), dim3(256), 0, stream, a, columns);

@@ -220,6 +220,10 @@ ATTENDS = [  # heads, kv heads, head size, page, rows of each request, tokens be
     (15, 5, 64, 16, [33], [0], 0),
     (2, 2, 96, 16, [40], [10], 100),
     (2, 1, 256, 16, [50], [40], 0),
+    (16, 16, 64, 16, [40, 0, 33], [960, 0, 100], 0),     # three tiles of columns a wave, of which some rows fill one and a half
+    (16, 16, 64, 32, [131, 5, 17], [1400, 20, 0], 1100),
+    (32, 32, 32, 16, [40], [1963], 0),
+    (24, 8, 32, 48, [90, 7], [1905, 0], 0),
 ]
 
 
