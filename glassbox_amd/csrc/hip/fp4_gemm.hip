@@ -418,6 +418,57 @@ __global__ __launch_bounds__(256) void fp4_gemm_join_kernel(GemmArgs a, int slic
   else ((float*)a.out)[o] = v;
 }
 
+// The same for a product that adds to the residual, a workgroup a row; with the new row in hand it does the RMS norm that reads it next as well:
+// h = bf16(gamma (x s)), s = 1 / sqrt(mean(x^2) + eps).  A thread has up to two words of four columns, whose slices it asks for eight at a time.  Bound by
+// the way into the few compute units that have a row.  us with the product, and with the norm in a launch of its own: 16 rows by 2,048 of 8,192 10.2 and 11.7, 64
+// 12.8 and 14.9, 512 33.0 and 36.5; 40 by 4,096 of 14,336 25.0 and 26.6, by 4,096 of 4,096 13.4 and 15.1.
+constexpr int kNormColumns = 2 * 4 * 1024;
+__global__ __launch_bounds__(1024) void fp4_gemm_join_norm_kernel(GemmArgs a, int slices) {
+  __shared__ float partial[16];
+  const int m = blockIdx.x, threads = blockDim.x;
+  const size_t step = (size_t)a.M * a.N;
+  f32x4 x[2];
+  float gamma[2][4], squares = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int n = 4 * ((int)threadIdx.x + i * threads);
+    if (n >= a.N) break;
+    const float* p = a.slices + (size_t)m * a.N + n;
+    f32x4* o = reinterpret_cast<f32x4*>((float*)a.out + (size_t)m * a.ldo + n);
+    const f32x4 old = *o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) gamma[i][e] = a.gamma32 ? ((const float*)a.gamma)[n + e] : (float)((const bf16*)a.gamma)[n + e];
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int z = 0; z < slices; z += 8) {
+      f32x4 v[8];   // (behind the last slice the last again, not added)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const f32x4*>(p + min(z + k, slices - 1) * step);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (z + k < slices) sum += v[k];
+    }
+    x[i] = old + sum;
+    *o = x[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) squares = fmaf(x[i][e], x[i][e], squares);
+  }
+  squares = wave_sum(squares);
+  if (threadIdx.x % kWave == 0) partial[threadIdx.x / kWave] = squares;
+  __syncthreads();
+  float total = 0.f;
+  for (int w = 0; w < threads / kWave; ++w) total += partial[w];
+  const float s = 1.f / sqrtf(total / a.N + a.eps);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int n = 4 * ((int)threadIdx.x + i * threads);
+    if (n >= a.N) break;
+    bf16x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (bf16)(gamma[i][e] * (x[i][e] * s));
+    *reinterpret_cast<bf16x4*>(a.h + (size_t)m * a.ldh + n) = y;
+  }
+}
+
 // Which kernel takes a product, and how: a function of its sizes and type alone.
 struct Form {
   int rows_w, rows_a, step;          // a workgroup's rows of W and of a, blocks of k a turn
@@ -505,7 +556,9 @@ template <typename T, int MT, int NT, int B> static void tiles(const Plan& p, co
   hipLaunchKernelGGL((fp4_tiles_kernel<T, MT, NT, B>), dim3((unsigned)((p.n_tiles + 7) / 8 * 8 * p.m_tiles), (unsigned)p.slices), dim3(256), 0, stream, a);
 }
 
-template <typename T> static void launch_by(const Plan& p, const GemmArgs& a, hipStream_t stream) {
+template <typename T> static void launch_by(const Plan& p, const GemmArgs& all, hipStream_t stream) {
+  GemmArgs a = all;
+  if (p.slices > 1) a.h = nullptr;   // (the pass behind the product does the norm)
   switch (p.form) {
     case 0: lines<T, 1, 4, 8, 1>(p, a, stream); break;
     case 1: lines<T, 1, 2, 8, 1>(p, a, stream); break;
@@ -525,7 +578,10 @@ template <typename T> static void launch_by(const Plan& p, const GemmArgs& a, hi
         else tiles<T, 4, 4, 4>(p, a, stream);
       }
   }
-  if (p.slices > 1) {
+  if (p.slices > 1 && all.h) {
+    const int threads = std::min(1024, (a.N / 4 + kWave - 1) / kWave * kWave);
+    hipLaunchKernelGGL(fp4_gemm_join_norm_kernel, dim3((unsigned)a.M), dim3(threads), 0, stream, all, p.slices);
+  } else if (p.slices > 1) {
     const long long cells = (long long)a.M * (a.epilogue == 2 ? a.N / 2 : a.N);
     hipLaunchKernelGGL(fp4_gemm_join_kernel, dim3((unsigned)((cells + 255) / 256)), dim3(256), 0, stream, a, p.slices);
   }
@@ -547,6 +603,14 @@ extern "C" int gb_fp4_gemm_emit_parts(int M, int N) {
   return M > 0 && M <= kNormRows && N > 0 && N % 8 == 0 ? plan(M, N, 32, false, kBF16, 1).n_tiles : 0;
 }
 
+// What a product that adds a.w to the residual can do for the norm behind it: 0 nothing; 1 partial sums (the tiles above); 2, where it divides k and
+// has its workspace, the whole norm (h given without sums).
+extern "C" int gb_fp4_gemm_emit_mode(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= kNormRows) return N % 8 == 0 ? 1 : 0;
+  return N % 4 == 0 && N <= kNormColumns && plan(M, N, K, false, kBF16, 16).slices > 1 ? 2 : 0;
+}
+
 // with what a product does for norms (GemmArgs)
 extern "C" int gb_fp4_gemm_norms(const void* x, int dtype, int ldx, const void* codes, const void* scales, int scale_stride, void* out, int out_dtype,
                                  int ldo, int M, int N, int K, int epilogue, float* workspace, long long workspace_floats, const void* gamma,
@@ -558,13 +622,15 @@ extern "C" int gb_fp4_gemm_norms(const void* x, int dtype, int ldx, const void* 
   GB_REQUIRE(scale_stride >= K / 32 && scale_stride % 16 == 0 && ((uintptr_t)codes & 15) == 0 && ((uintptr_t)scales & 15) == 0,
              "fp4_gemm: codes and scales begin at 16-byte words, rows of scales are multiples of 16");
   GB_REQUIRE((dtype == kF32 || dtype == kBF16) && (out_dtype == kF32 || out_dtype == kBF16), "fp4_gemm: unknown dtype %d or %d", dtype, out_dtype);
-  GB_REQUIRE(!h || (dtype == kBF16 && epilogue == 1 && M <= kNormRows && N % 8 == 0 && (uintptr_t)out % 16 == 0 && ldo % 4 == 0 && (uintptr_t)h % 8 == 0 &&
-                    ldh % 4 == 0 && ldh >= N && sums && gamma && (gamma_dtype == kF32 || gamma_dtype == kBF16)),
-             "fp4_gemm: a norm is prepared by products that add up to %d bfloat16 rows, of a multiple of 8 columns in whole words", kNormRows);
+  GB_REQUIRE(!h || (dtype == kBF16 && epilogue == 1 && M <= (sums ? kNormRows : INT32_MAX) && N % (sums ? 8 : 4) == 0 && (uintptr_t)out % 16 == 0 && ldo % 4 == 0 &&
+                    (uintptr_t)h % 8 == 0 && ldh % 4 == 0 && ldh >= N && gamma && (gamma_dtype == kF32 || gamma_dtype == kBF16)),
+             "fp4_gemm: a norm is prepared by products that add bfloat16 rows (up to %d, or with k divided), of a multiple of 8 (4) columns in whole words",
+             kNormRows);
   GB_REQUIRE(!parts || (dtype == kBF16 && epilogue != 1 && M <= kNormRows && n_parts > 0 && n_parts < (1 << 24) && (uintptr_t)parts % 16 == 0), "fp4_gemm: a norm's sums go with up to %d bfloat16 rows", kNormRows);
   if (M == 0) return 0;
   Plan p = plan(M, N, K, epilogue == 2, dtype, 16);
   if (p.slices > 1 && (!workspace || workspace_floats < (long long)p.slices * M * N)) p = plan(M, N, K, epilogue == 2, dtype, 1);   // slower, not refused
+  GB_REQUIRE(!h || sums || (p.slices > 1 && N <= kNormColumns), "fp4_gemm: a norm of rows whose product does not divide k, or of more than %d columns", kNormColumns);
   GB_REQUIRE((long long)(p.n_tiles + 7) * p.m_tiles < (1ll << 31) && (long long)M * N < (1ll << 38), "fp4_gemm: %d x %d is too much for one launch", M, N);
   const int e = out_dtype == kF32 ? 16 : 8;   // bytes of four columns
   const GemmArgs a{x, (const uint8_t*)codes, (const uint8_t*)scales, out, p.slices > 1 ? workspace : nullptr, parts, gamma,

@@ -2830,6 +2830,16 @@ def fp4_gemm_emit_parts(rows: int, n: int) -> int:
     return int(_lib("fp4_gemm").gb_fp4_gemm_emit_parts(int(rows), int(n)))
 
 
+@functools.lru_cache(maxsize=4096)   # a pure function of the sizes, asked for at every product
+def fp4_gemm_emit_mode(rows: int, n: int, k: int) -> int:
+    """What an accumulating product of ``rows`` bfloat16 rows and ``n`` rows of w of ``k`` numbers can do for the RMS norm that reads the residual
+    after it, as ``gemm_emit_mode`` says of ``gemm``: 0 nothing; 1 the operand and partial sums (``fp4_gemm(..., emit=(gamma, h, parts))``); 2 the whole
+    norm (``fp4_gemm(..., emit=(gamma, h, eps), workspace=...)``: h receives the normed rows)."""
+    if _fp4_expands(rows, n, k, torch.bfloat16, torch.float32, False):
+        return 0
+    return int(_lib("fp4_gemm").gb_fp4_gemm_emit_mode(int(rows), int(n), int(k)))
+
+
 def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool = False, silu_mul: bool = False,
              workspace: Optional[torch.Tensor] = None, emit: Optional[tuple] = None, rms_parts: Optional[tuple] = None) -> None:
     """out (+)= a . w^T with four-bit weights, the sums in 32 bits: ``a`` [rows, columns of w] bfloat16 or float32, ``out`` bfloat16 or float32
@@ -2837,7 +2847,8 @@ def fp4_gemm(a: torch.Tensor, w: Fp4Matrix, out: torch.Tensor, accumulate: bool 
     many columns.
     ``emit=(gamma, h, parts)`` (accumulating, bfloat16 rows, where ``fp4_gemm_emit_parts`` is not 0): besides the new residual r in out,
     h[m, n] = bf16(gamma[n] r[m, n]) and float32 parts[tile, m] of sum(r^2) over the tile's columns are written (``parts_stride(M)`` floats a tile), as
-    ``gemm`` does.  ``rms_parts=(parts, n_parts, eps)`` (up to 8 rows): a is such an h, and the product is scaled to that of the normed rows.
+    ``gemm`` does.  ``emit=(gamma, h, eps)`` with a number as the third entry (where ``fp4_gemm_emit_mode`` is 2, with the workspace): h receives the rows of
+    that norm itself, bf16(gamma * r / sqrt(mean(r^2) + eps)).  ``rms_parts=(parts, n_parts, eps)`` (up to 8 rows): a is such an h, and the product is scaled to that of the normed rows.
     ``workspace`` (float32, ``fp4_gemm_floats`` elements; optional): lets few workgroups divide k (their sums are added in a fixed order), and
     large bfloat16 products have the weights' bfloat16 values written there first and multiplied by ``gemm``."""
     N, K, each, c_at, s_at = _fp4_matrix(w, "fp4_gemm")
@@ -2873,10 +2884,13 @@ def _fp4_gemm_norms(a, w, out, args: tuple, workspace, emit: Optional[tuple], rm
     n_parts, eps, ldh = 0, 0.0, 0
     if emit is not None:
         gamma, h, sums = emit
-        if (not accumulate or dtype != BF16 or M > 8 or N % 8 or gamma.numel() != N or not gamma.is_contiguous() or h.dtype != torch.bfloat16
-                or h.shape != out.shape or sums.dtype is not _FLOAT or not sums.is_contiguous()):
-            raise KernelError("fp4_gemm: emit needs an accumulating product that fp4_gemm_emit_parts accepts, gamma of N entries, a bfloat16 [M, N] "
-                              "operand buffer and float32 parts")
+        whole = not isinstance(sums, torch.Tensor)
+        if whole:
+            sums, eps = None, float(sums)
+        if (not accumulate or dtype != BF16 or (M <= 8 or N % 4 if whole else M > 8 or N % 8) or gamma.numel() != N or not gamma.is_contiguous() or h.dtype != torch.bfloat16
+                or h.shape != out.shape or not whole and (sums.dtype is not _FLOAT or not sums.is_contiguous())):
+            raise KernelError("fp4_gemm: emit needs an accumulating product that fp4_gemm_emit_parts or fp4_gemm_emit_mode accepts, gamma of N entries, a "
+                              "bfloat16 [M, N] operand buffer and float32 parts, or eps")
         ldh, at, lda, to, ldo = _rows(h, "emit h"), args[0], args[2], args[6], args[8]
         if M and not (_apart(h.data_ptr(), M, 2 * N, 2 * ldh, at, M, 2 * args[11], 2 * lda) and _apart(h.data_ptr(), M, 2 * N, 2 * ldh, to, M, 4 * N, 4 * ldo)):
             raise KernelError("fp4_gemm: the rows of emit share memory with a or out")
@@ -2888,6 +2902,8 @@ def _fp4_gemm_norms(a, w, out, args: tuple, workspace, emit: Optional[tuple], rm
     here = _here("fp4_gemm", a, w[0], w[1], out, workspace, gamma, h, sums, parts)
     if sums is not None and sums.numel() < fp4_gemm_emit_parts(M, N) * parts_stride(M):
         raise KernelError(f"fp4_gemm: emit needs parts_stride(M) float32 for each of {fp4_gemm_emit_parts(M, N)} parts, {sums.numel()} are given")
+    if emit is not None and sums is None and (fp4_gemm_emit_mode(M, N, args[11]) != 2 or args[14] < fp4_gemm_floats(M, N, args[11], a.dtype, out.dtype)):
+        raise KernelError("fp4_gemm: a norm is finished by products that divide k (fp4_gemm_emit_mode 2), with their workspace")
     lib = _lib("fp4_gemm")
     _launch(lib, lib.gb_fp4_gemm_norms, *args, _p(gamma), 0 if gamma is None else dtype_code(gamma), _p(h), ldh, _p(sums), _p(parts), n_parts, eps,
             _stream_of(here))

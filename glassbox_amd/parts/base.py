@@ -182,7 +182,7 @@ def needs_multiple_of_32(what: str, size: int) -> List[str]:
 def fp4_product(ctx, a, codes, scales, out, accumulate: bool = False, silu_mul: bool = False, norm=None, emit=None, tag: str = ""):
     """``ops.fp4_gemm`` with the workspace that it has a use for in this step.  ``norm``: a is the residual before this norm, ``(gamma, eps)``,
     or what a product before it prepared of it (``PreNormed``).  ``emit=(gamma, eps)``: the product, which adds into the residual, may prepare
-    the norm that reads it next; returns a PreNormed if it did."""
+    the norm that reads it next, or do it; returns a PreNormed or Normed if it did."""
     from .. import ops
     n, w, more, handed_on = a.shape[0], ops.Fp4Matrix(codes, scales), {}, None
     if isinstance(norm, PreNormed):
@@ -191,11 +191,15 @@ def fp4_product(ctx, a, codes, scales, out, accumulate: bool = False, silu_mul: 
         a, x = ctx.buffer("h", tuple(a.shape), ctx.dtype), a
         ops.rmsnorm(x, norm[0], norm[1], a)
     if emit is not None and ctx.fuse_norms and a.dtype == torch.bfloat16:
-        n_parts = ops.fp4_gemm_emit_parts(n, codes.shape[0])
-        if n_parts:
+        mode = ops.fp4_gemm_emit_mode(n, codes.shape[0], a.shape[1])
+        if mode == 1:
+            n_parts = ops.fp4_gemm_emit_parts(n, codes.shape[0])
             rows = ctx.buffer(f"prenorm_rows_{tag}", tuple(out.shape), torch.bfloat16)
             parts = ctx.buffer(f"prenorm_parts_{tag}", (n_parts, ops.parts_stride(n)), torch.float32)
             more["emit"], handed_on = (emit[0], rows, parts), PreNormed(rows, parts, n_parts, float(emit[1]))
+        elif mode == 2:
+            rows = ctx.buffer(f"normed_rows_{tag}", tuple(out.shape), torch.bfloat16)
+            more["emit"], handed_on = (emit[0], rows, float(emit[1])), Normed(rows)
     floats = ops.fp4_gemm_floats(n, codes.shape[0], a.shape[1], a.dtype, out.dtype, silu_mul)
     ops.fp4_gemm(a, w, out, accumulate=accumulate, silu_mul=silu_mul, workspace=ctx.buffer("fp4_gemm", (floats,), torch.float32) if floats else None,
                  **more)

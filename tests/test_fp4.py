@@ -78,6 +78,7 @@ REFUSED = [
     (gemm, dict(ADDS, emit=(torch.ones(10), torch.zeros(3, 10, dtype=BF), torch.zeros(8, 8))), "emit needs"),           # 10 columns
     (gemm, dict(ADDS8, accumulate=False, emit=EMIT), "emit needs"), (gemm, dict(ADDS8, a=torch.zeros(3, 64), emit=EMIT), "emit needs"),
     (gemm, dict(ADDS8, emit=(torch.ones(15), *EMIT[1:])), "emit needs"), (gemm, dict(ADDS8, emit=(EMIT[0], torch.zeros(3, 16), EMIT[2])), "emit needs"),
+    (gemm, dict(ADDS8, emit=(*EMIT[:2], 1e-5)), "emit needs"),                                                          # the whole norm of 3 rows
     (gemm, dict(ADDS8, emit=(*EMIT[:2], torch.zeros(8, 8, dtype=BF))), "emit needs"), (gemm, dict(ADDS8, emit=EMIT), "current GPU"),
     (gemm, dict(ADDS8, a=torch.zeros(9, 64, dtype=BF), out=torch.zeros(9, 16), emit=(EMIT[0], torch.zeros(9, 16, dtype=BF), torch.zeros(8, 64))), "emit needs"),
     (gemm, dict(ADDS8, a=ROWS[:3, :64], emit=(EMIT[0], ROWS[:3, 60:76], EMIT[2])), "share memory"),

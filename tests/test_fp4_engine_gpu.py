@@ -221,3 +221,32 @@ def test_a_window_and_a_layer_that_reads_another_ones_cache(packed):
     want = (plain.rms_norm(x, w["model.norm.weight"], eps) @ w["model.embed_tokens.weight"].T).numpy()
     bad = helpers.first_bad(np.asarray(got), want, helpers.TOL_F32)
     assert bad is None, f"position {bad[0]} off by {bad[1]:.3e}"
+
+
+def test_norms_that_the_products_do_are_those_of_their_own_launch(monkeypatch):
+    """Rows whose squares' sums are exact, so that their order does not matter: the first layer adds nothing to an embedding of halves."""
+    from glassbox_amd import ops
+    from glassbox_amd.config import config_from_dict
+    from glassbox_amd.engine import Engine
+    from glassbox_amd.weights import build_model
+    from glassbox_amd.weights.loader import random_tensors
+    d, inter, vocab = 1056, 8224, 90
+    cfg = config_from_dict(dict(helpers.TINY_B, hidden_size=d, intermediate_size=inter, num_hidden_layers=2, num_attention_heads=4,
+                                num_key_value_heads=2, head_dim=64, vocab_size=vocab))
+    model = build_model(cfg)
+    tensors = random_tensors(model, 7, 0.1, "uniform", torch.bfloat16, "cuda:0")
+    for name in ("self_attn.o_proj", "mlp.down_proj"):
+        tensors[f"model.layers.0.{name}.weight"].zero_()
+    tensors["model.embed_tokens.weight"].copy_(torch.randint(-3, 4, (vocab, d), generator=torch.Generator().manual_seed(3)) * 0.5)
+    model.load_tree(tensors)
+    asked, mode = [], ops.fp4_gemm_emit_mode
+    got = []
+    for on in (True, False):
+        monkeypatch.setattr(ops, "fp4_gemm_emit_mode", lambda m, n, k: (asked.append((m, mode(m, n, k))), mode(m, n, k))[1] if on else 0)
+        eng = Engine(model, dtype="bfloat16", max_tokens=1024, max_seqs=48, kv_cache="fp4", weights="fp4")
+        first = eng.step([("r", helpers.random_tokens(vocab, 33, 1), list(range(33)))]).clone()
+        got.append([first] + [eng.step([((m, i), [3 * i % vocab], [0]) for i in range(m)])[:m].clone() for m in (12, 32)])
+        del eng
+    assert {(33, 2), (32, 2)} <= set(asked)
+    for mine, apart in zip(*got):
+        assert mine.isfinite().all() and torch.equal(mine[:, :vocab], apart[:, :vocab])

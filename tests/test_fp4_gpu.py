@@ -621,3 +621,40 @@ def test_a_product_prepares_a_norm_and_the_next_takes_it(M, N, K, gamma_dtype):
         g, u, dg, du = y[:, :C // 2], y[:, C // 2:], off[:, :C // 2], off[:, C // 2:]
         z, dz = g * torch.sigmoid(g) * u, 1.1 * dg * (u.abs() + du) + (g.abs() + dg) * du + 8 * STEP * (g * u).abs()
         assert ((out.double() - z).abs() <= dz + half_step(out_dtype) * (z.abs() + dz) + 1e-30).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(30, 1040, 8224), (64, 4100, 4128), (65, 6148, 4128), (700, 68, 4128), (9, 2052, 8224), (520, 260, 8224), (12, 8192, 8192)])
+@pytest.mark.parametrize("gamma_dtype", [torch.float32, torch.bfloat16])
+def test_a_product_that_divides_k_does_the_norm(M, N, K, gamma_dtype):
+    from glassbox_amd import ops
+    assert ops.fp4_gemm_emit_mode(M, N, K) == 2
+    w = ops.fp4_quantize(normal(N, K, seed=70, scale=0.05).to(DEV))
+    a, first = normal(M, K, seed=71, wide=4.0).bfloat16().to(DEV), normal(M, N, seed=72, wide=3.0).to(DEV)
+    gamma, eps = (normal(N, seed=73) + 1).to(gamma_dtype).to(DEV), 1e-5
+    x, plain_x = torch.full((M, N + 4), 5.0, device=DEV), first.clone()
+    x[:, :N] = first
+    h = torch.full((M, N + 8), 3.0, dtype=torch.bfloat16, device=DEV)
+    ws = torch.full((ops.fp4_gemm_floats(M, N, K, torch.bfloat16, torch.float32) + 16,), math.nan, device=DEV)
+    for few in (None, ws[:-17]):
+        with pytest.raises(ops.KernelError, match="divide k"):
+            ops.fp4_gemm(a, w, x[:, :N], accumulate=True, emit=(gamma, h[:, :N], eps), workspace=few)
+    ops.fp4_gemm(a, w, x[:, :N], accumulate=True, emit=(gamma, h[:, :N], eps), workspace=ws[:-16])
+    ops.fp4_gemm(a, w, plain_x, accumulate=True, workspace=ws[:-16])
+    assert torch.equal(x[:, :N], plain_x) and (x[:, N:] == 5).all() and (h[:, N:] == 3).all() and ws[-16:].isnan().all()
+    rows = plain_x.double()
+    want = gamma.double() * rows / torch.sqrt((rows ** 2).mean(-1, keepdim=True) + eps)
+    # up to 8 numbers a thread, 6 exchanges and 16 waves make a row's sum, each a rounding of what is positive: half of that in its root; and a quotient, two
+    # roots' and quotients' roundings, two products
+    off = (15 + 8) * STEP * want.abs()
+    assert ((h[:, :N].double() - want).abs() <= off + half_step(torch.bfloat16) * (want.abs() + off) + 1e-30).all()
+
+
+def test_a_norm_is_refused_where_a_product_does_not_divide_k():
+    from glassbox_amd import ops
+    M, N, K = 33, 36, 4128
+    assert ops.fp4_gemm_emit_mode(M, N, K) == 0 and ops.fp4_gemm_emit_mode(0, N, K) == 0 and ops.fp4_gemm_emit_mode(12, 8196, 8192) == 0
+    w, x = ops.fp4_quantize(torch.ones(N, K, device=DEV)), torch.zeros(M, N, device=DEV)
+    with pytest.raises(ops.KernelError, match="divide k"):
+        ops.fp4_gemm(torch.ones(M, K, dtype=torch.bfloat16, device=DEV), w, x, accumulate=True, workspace=torch.zeros(1 << 20, device=DEV),
+                     emit=(torch.ones(N, device=DEV), torch.zeros(M, N, dtype=torch.bfloat16, device=DEV), 1e-5))
+    assert (x == 0).all()
