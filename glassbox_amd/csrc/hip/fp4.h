@@ -122,6 +122,16 @@ __device__ __forceinline__ void fp4_terms(const float (&x)[8], bf16x8 (&out)[3])
     __builtin_memcpy(&out[k], w, sizeof w);
   }
 }
+// Probabilities as two bf16 numbers: the upper eight bits of the mantissa, and the nearest to what is left, together
+// off by at most 2^-16 of the number.
+__device__ __forceinline__ void fp4_terms(const float (&x)[8], bf16x8 (&out)[2]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) out[1][i] = (bf16)(x[i] - __uint_as_float(__float_as_uint(x[i]) & 0xffff0000u));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1]), __float_as_uint(x[2 * i]), 0x07060302u);
+  __builtin_memcpy(&out[0], w, sizeof w);
+}
 __device__ __forceinline__ void fp4_terms(const float (&x)[8], bf16x8 (&out)[1]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) out[0][i] = (bf16)x[i];

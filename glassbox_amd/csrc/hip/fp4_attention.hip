@@ -13,8 +13,9 @@
 //            (r, r + 16) of a block are 16 consecutive bytes, and their scales 16 more.
 //
 // Codes become bf16 in registers, two an instruction with their scale, exactly; nothing passes through LDS but the joining of waves.
-// A row of 32 bits counts as three bf16 terms (fp4.h), and so do its probabilities; a bf16 row's probabilities are rounded to bf16, as
-// its result is.
+// A row of 32 bits counts as three bf16 terms (fp4.h), and so do its probabilities.  Those of a bf16 row count as two, off by 2^-16: its
+// result is rounded once, at the end.  (As one term they were off by 2^-8: the distance from the 64-bit definition was 0.0021 of the results where their
+// own rounding is 0.0016, and far more of sums that cancel; it took 4 to 6 % less time for single tokens, 12 to 17 % less for portions.)
 //
 // Few columns (decoding): the waves of a workgroup share out the tiles and are joined through LDS; a long context is cut into runs
 // for several workgroups, joined by a second kernel.  More columns: each wave has columns of its own and all of a run's keys.
@@ -128,10 +129,10 @@ __device__ __forceinline__ uint32_t mask_scores(f32x4 (&sc)[4], int key, bool kn
 }
 
 // One step of the running softmax of a column (this lane's 16 keys of 64): probabilities as the product's operand, sums rescaled where
-// the maximum grows.  Their sum is a product with ones, of what the values are multiplied by and over all 64 (added up by the lanes: 2,048 rows of 32
-// heads of 128 62.6 us for 60.6, 131 rows behind 3,900 26.7 for 26.2, two tiles a wave).
-template <int SP, int NB>
-__device__ __forceinline__ void soften(const f32x4 (&sc)[4], float scale, float& m, f32x4& l, f32x4 (&o)[2 * NB], bf16x8 (&pf)[SP][2]) {
+// the maximum grows.  Their sum is a product with ones, of what the values are multiplied by and over all 64 (added up by the lanes: 64 requests of
+// 4,096 keys 136 us for 126, 2,048 rows of 32 heads of 128 72.5 for 73).  PT terms a probability.
+template <int PT, int NB>
+__device__ __forceinline__ void soften(const f32x4 (&sc)[4], float scale, float& m, f32x4& l, f32x4 (&o)[2 * NB], bf16x8 (&pf)[PT][2]) {
   float top = -__builtin_inff();
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -158,10 +159,10 @@ __device__ __forceinline__ void soften(const f32x4 (&sc)[4], float scale, float&
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = p[8 * c + e];
-    bf16x8 terms[SP];
+    bf16x8 terms[PT];
     fp4_terms(x, terms);
 #pragma unroll
-    for (int q = 0; q < SP; ++q) {
+    for (int q = 0; q < PT; ++q) {
       pf[q][c] = terms[q];
       l = mfma(bf16x8{} + (bf16)1.f, terms[q], l);
     }
@@ -243,7 +244,7 @@ template <int NB> __device__ __forceinline__ void load_tile(const AttendArgs& a,
 // R tiles of 16 columns over a tile of keys: their scores, the step of their softmax, their sums.  first, last: the columns' positions;
 // [lo, end): keys that some column may see.
 template <typename T, int NB, int R> struct Columns {
-  static constexpr int SP = kFp4Terms<T>;
+  static constexpr int SP = kFp4Terms<T>, PT = SP > 1 ? SP : 2;
   bf16x8 qf[R][SP][NB];
   f32x4 o[R][2 * NB];
   float m[R];
@@ -302,9 +303,9 @@ template <typename T, int NB, int R> struct Columns {
       }
       bad = __any(any != 0);
     }
-    bf16x8 pf[R][SP][2];
+    bf16x8 pf[R][PT][2];
 #pragma unroll
-    for (int t = 0; t < R; ++t) soften<SP, NB>(sc[t], a.scale, m[t], l[t], o[t], pf[t]);
+    for (int t = 0; t < R; ++t) soften<PT, NB>(sc[t], a.scale, m[t], l[t], o[t], pf[t]);
     if (__builtin_expect(bad, 0)) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
@@ -326,9 +327,9 @@ template <typename T, int NB, int R> struct Columns {
         bf16x8 low, high;
         values8(w.vw[b][2 * c], w.vw[b][2 * c + 1], w.vs[b][2 * c], w.vs[b][2 * c + 1], low, high);
 #pragma unroll
-        for (int t = 0; t < R; ++t)
+        for (int p = 0; p < PT; ++p)
 #pragma unroll
-          for (int p = 0; p < SP; ++p) {
+          for (int t = 0; t < R; ++t) {
             o[t][2 * b] = mfma(low, pf[t][p][c], o[t][2 * b]);
             o[t][2 * b + 1] = mfma(high, pf[t][p][c], o[t][2 * b + 1]);
           }
@@ -336,12 +337,12 @@ template <typename T, int NB, int R> struct Columns {
   }
 };
 
-// Waves a SIMD holds at least: what just fits the registers.  (Without the bound a few more registers cost a wave: 40 requests of 8,000 keys 63 us, with
-// it 59.)
+// Waves a SIMD holds at least: what just fits the registers.  (Without the bound a few more registers cost a wave: 64 requests of 4,096 keys, 32 heads of
+// 64, 158 us, with it 127; 2,048 rows of 32 heads of 128 108 and 73.)
 template <typename T, int NB, int R> constexpr int least_waves = NB > 4 ? 1 : std::is_same_v<T, float> || R > 1 ? 2 : NB > 2 ? 3 : 4;
 
 // Few columns: the waves of a workgroup share out the tiles of keys.  T the rows' type, NB blocks a head, W waves.  Bound by memory: 64 requests of
-// 4,096 keys, 32 heads of 64, 119 us for 571 MB (4.8 TB/s); 64 of 4,000, 8 kv heads of 128, 59 us (4.7 TB/s).
+// 4,096 keys, 32 heads of 64, 127 us for 571 MB (4.5 TB/s); 64 of 4,000, 8 kv heads of 128, 62 us (4.5 TB/s).
 template <typename T, int NB, int W>
 __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least_waves<T, NB, 1>))) void fp4_attend_keys_kernel(AttendArgs a) {
   constexpr int D = NB * kFp4Block;
@@ -371,7 +372,6 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least
     const bool known = known_page(a, at.vp);
     Tile<NB> tile;
     load_tile(a, at, kvh, r, g, tile);
-    __builtin_amdgcn_sched_barrier(0);   // (all of a tile is asked for before anything is computed: 62.8 us without, 61.8 with)
     at = look_up(a, table, t0 + W * kTile + 16 * (r >> 2), t0 + W * kTile + 16 * g);
     columns.take(a, tile, t0, known, first, last, lo, end, g);
   }
@@ -413,10 +413,10 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least
   }
 }
 
-// More columns: each of four waves has R tiles of its own and takes all keys.  Bound by the conversions and the softmax: 2,048 rows of 32 heads of
-// 128 in 60.6 us (the same rows over a bf16 cache in the prefill kernel: 56).  A request's long tiles of columns come first and its short ones
-// behind them in turn, so that compute units of two workgroups have about the same to do: in their order 84.  Making a tile bf16 once for the
-// four waves, through LDS, took 95: the barriers cost more than the conversions that they save.
+// More columns: each of four waves has R tiles of its own and takes all keys.  Bound by the conversions, the softmax and the products, which add up: 2,048
+// rows of 32 heads of 128 in 73 us (the same rows over a bf16 cache in the prefill kernel: 56).  A request's long tiles of columns come first and its
+// short ones behind them in turn, so that compute units of two workgroups have about the same to do: in their order 93.  Making a tile bf16 once for
+// the four waves, through LDS, took half as long again (95 for 64, with probabilities of one term): the barriers cost more than the conversions that they save.
 template <typename T, int NB, int R>
 __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(least_waves<T, NB, R>))) void fp4_attend_cols_kernel(AttendArgs a) {
   constexpr int D = NB * kFp4Block, C = 16 * R;
@@ -521,9 +521,9 @@ static Plan plan(int n_seqs, int nkv, int rep, int hd, int max_q, int max_contex
     return Plan{cols, r, (int)((columns + width - 1) / width), (int)std::max<long long>(1, (span + chunk - 1) / chunk), (int)chunk};
   };
   // Few columns, runs of a context: as many workgroups as compute units have one, none of fewer than 512 keys; 129 to 217 workgroups of long contexts
-  // in three.  Over 110 sizes 1.6 % slower than the best number of runs.  us: one request of 4,000 keys and 32 kv heads in 8 runs 9.5, in 4 11;
-  // 256 workgroups in one run 18.2, in two 21.9; 160 (5 of 9,000) in three 28.4, in two 35.5.  More than 256 stay whole: 40 requests of 1,000 to 8,000 keys
-  // and 8 kv heads 61.6, in three 65.4, though 10 of 9,000 and 32 kv heads take 58 and 47.
+  // in three.  Over 110 sizes 1.6 % slower than the best number of runs.  us: one request of 4,000 keys and 32 kv heads in 8 runs 9.8, in 4 11.3;
+  // 256 workgroups in one run 20.0, in two 23.3; 160 (5 of 9,000) in three 30.5, in two 39.3.  More than 256 stay whole: 40 requests of 1,000 to 8,000 keys
+  // and 8 kv heads 65.8, in three 66.4, though 10 of 9,000 and 32 kv heads take 65.7 and 52.5.
   if (columns <= 32) {
     const long long groups = (long long)n_seqs * nkv * ((columns + 15) / 16);
     long long runs = std::max<long long>(1, std::min<long long>(256 / groups, kMostSplits));
@@ -532,11 +532,11 @@ static Plan plan(int n_seqs, int nkv, int rep, int hd, int max_q, int max_contex
     return laid_out(false, 1, runs, 512, 8 * kTile);
   }
   // More: one tile of columns a wave, two (where they fit the registers) or three (heads of 64: of 32 they gain nothing), and as many runs, as take least by a model with numbers fitted to some 2,000
-  // launches (70 sizes, 9 % off; its choice is 3 % slower than the best, at most 18): a wave's turns, each `alone` us; the tiles that a SIMD has to do on
-  // average, `busy` us each, more where the workgroups do not divide evenly by the compute units; the joining of runs, its launch and its
-  // bytes.  us: 131 rows behind 3,900, 32 heads of 64 and as many kv heads, three tiles in 8 runs 24.3, two in 11 26.6, one in 8 30.2; 8 kv heads of 128 two
-  // in 6 33.4, in 8 38.6; 1,024 rows of 32 heads of 64 two in one run 23, in two 43; 8 x 50 rows behind 550 one in one 16, two in three 25;
-  // 131 rows behind 15,869, 32 heads of 64, three in 16 52, two in 10 59; 300 behind 15,700 91 and 104.
+  // launches (of probabilities of one term; its choice is 3 % slower than the best over 64 sizes, at most 20): a wave's turns, each `alone` us; the tiles that a
+  // SIMD has to do on average, `busy` us each, more where the workgroups do not divide evenly by the compute units; the joining of runs, its launch and its
+  // bytes.  us: 131 rows behind 3,900, 32 heads of 64 and as many kv heads, three tiles in 8 runs 27.1, two in 11 27.9, one in 11 33.4; 8 kv heads of 128 two
+  // in 6 36.3, in 8 43.7; 1,024 rows of 32 heads of 64 two in one run 27.4, in two 42.3, though one in one takes 22.9; 8 x 50 rows behind 550 one in one
+  // 22.6, two in two 29.1; 131 rows behind 15,869, 32 heads of 64, three in 23 65.4, two in 16 76.7; 300 behind 15,700 three in 12 115, two in 16 124.
   static constexpr float kAlone[3][9] = {{0.f, 0.38f, 0.48f, 1.2f, 0.75f, 0.f, 0.f, 0.f, 1.f}, {0.f, 0.55f, 0.59f, 1.35f, 1.01f}, {0.f, 0.f, 0.89f}};   // by tiles and blocks a head
   static constexpr float kBusy[3][9] = {{0.f, 0.52f, 0.65f, 1.1f, 0.84f, 0.f, 0.f, 0.f, 2.2f}, {0.f, 0.59f, 0.8f, 1.2f, 0.91f}, {0.f, 0.f, 0.9f}};
   const bool wide = dtype == kF32;
