@@ -82,7 +82,8 @@ def check_four_bits(model, kv_cache: Optional[str], weights: Optional[str]) -> N
     lines = []
     if kv_cache == "fp4":
         heads = ", ".join(map(str, ops.FP4_HEAD_DIMS))
-        lines += [f"kv_cache='fp4': cache layer {c}: four-bit pages are for plain attention with heads of {heads} channels"
+        lines += [f"kv_cache='fp4': cache layer {c}: four-bit pages are for plain attention with heads of {heads} channels and a position "
+                  f"encoding that leaves the cache write to others (PositionEncoding.fuse_spec or apply)"
                   for c, spec in enumerate(model.cache_specs()) if spec is not None and not spec.four_bits]
     if weights == "fp4":
         lines += [f"weights='fp4': {line}" for line in model.four_bit_obstacles()]

@@ -91,7 +91,7 @@ class PagedAttention(Mixer):
         self.q_dim = n_heads * head_dim
         self.kv_dim = n_kv_heads * head_dim
         self.cache_spec = None if shares_kv else CacheSpec(n_kv_heads, head_dim, WINDOW if window > 0 else FULL, self.window,
-                                                           four_bits=head_dim in ops.FP4_HEAD_DIMS)
+                                                           four_bits=head_dim in ops.FP4_HEAD_DIMS and position.leaves_the_store())
         self.wqkv: Optional[torch.Tensor] = None          # (four-bit codes, with the scales below, after ``quantize``)
         self.wo: Optional[torch.Tensor] = None
         self.wqkv_scales: Optional[torch.Tensor] = None
@@ -218,7 +218,10 @@ class PagedAttention(Mixer):
         if cache.k_pages.dtype == torch.uint8:
             angles = self.position.fuse_spec(ctx, self.head_dim)
             if angles is None:   # an encoding that does its own work does it in place; the heads are then stored as they are
-                self.position.apply_and_store(ctx, qkv, self.n_heads, n_kv, self.head_dim, None, None, None)
+                if slots is None:
+                    self.position.apply_and_store(ctx, qkv, self.n_heads, n_kv, self.head_dim, None, None, None)
+                else:
+                    self.position.apply(ctx, qkv, self.n_heads, n_kv, self.head_dim)
                 angles = (None, None)
             ops.fp4_store(qkv, *angles, slots, cache.k_pages, cache.v_pages, self.n_heads, n_kv, self.head_dim)
             fp4_paged_attention(ctx, qkv[:, :self.q_dim], att, cache, self.n_heads, self.scale, self.window)

@@ -13,6 +13,8 @@ Interfaces (all activations are [tokens, width] tensors on the device;
   PositionEncoding.apply_and_store(ctx, qkv, n_heads, n_kv_heads, head_dim, slots, k_pages, v_pages)
                                                     encodes positions into the query/key heads of the
                                                     stacked rows in place and writes keys/values to pages
+  PositionEncoding.apply(ctx, qkv, n_heads, n_kv_heads, head_dim)
+                                                    the same without the write (optional: four-bit pages)
   Mixer.forward(ctx, h, residual, cache)            adds the mixed rows into ``residual`` (float32)
       .cache_spec  -> CacheSpec | None              paged keys/values it needs
       .state_spec  -> StateSpec | None              fixed-size per-request state it needs
@@ -231,7 +233,19 @@ class Norm(Part):
 
 class PositionEncoding(Part):
     def apply_and_store(self, ctx, qkv, n_heads, n_kv_heads, head_dim, slots, k_pages, v_pages) -> None:
+        """Encodes the heads in place and writes keys and values to the pages at ``slots``; with ``slots`` None nothing is
+        stored, and key heads may be left as they are."""
         raise NotImplementedError
+
+    def apply(self, ctx, qkv, n_heads, n_kv_heads, head_dim) -> None:
+        """Encodes query and key heads in place and stores nothing: for pages that a kernel of their own writes (four
+        bits).  Asked for where ``fuse_spec`` gives None."""
+        raise NotImplementedError(f"{type(self).__name__} encodes keys only on their way into pages of the compute type")
+
+    def leaves_the_store(self) -> bool:
+        """Whether encoded keys can be had without the cache write of ``apply_and_store``: pages of four bits need it."""
+        mine = type(self)
+        return mine.fuse_spec is not PositionEncoding.fuse_spec or mine.apply is not PositionEncoding.apply
 
     def fuse_spec(self, ctx, head_dim: int):
         """``(cos, sin)`` tables of the step's rows (float32 ``[n, head_dim/2]``; ``(None, None)`` for no

@@ -76,6 +76,8 @@ class Rotary(PositionEncoding):
         ops.rope_store(qkv, cos, sin, slots, k_pages, v_pages, n_heads, n_kv_heads, head_dim, rotate=True,
                        portions=ctx.portions())
 
+    def apply(self, ctx, qkv, n_heads, n_kv_heads, head_dim):
+        self.apply_and_store(ctx, qkv, n_heads, n_kv_heads, head_dim, None, None, None)   # (this one turns the keys all the same)
 
     def fuse_spec(self, ctx, head_dim: int):
         return self.table(ctx) if head_dim == self.head_dim and self.magnitude == 1.0 else None
@@ -88,6 +90,9 @@ class NoPosition(PositionEncoding):
 
     def fuse_spec(self, ctx, head_dim: int):
         return (None, None)
+
+    def apply(self, ctx, qkv, n_heads, n_kv_heads, head_dim):
+        pass
 
     def apply_and_store(self, ctx, qkv, n_heads, n_kv_heads, head_dim, slots, k_pages, v_pages):
         if slots is not None:
