@@ -79,6 +79,12 @@ def check_four_bits(model, kv_cache: Optional[str], weights: Optional[str]) -> N
     for name, value in (("kv_cache", kv_cache), ("weights", weights)):
         if value not in (None, "fp4"):
             raise EngineError(f"{name}={value!r}: None (the compute type) or 'fp4' (four bits)")
+    if weights is None and getattr(model, "quantized", False):
+        raise EngineError("weights=None: the matrices of this model are held in four bits already (an engine before, or quantize(), did that in "
+                          "place): ask for weights='fp4', or load the weights into another model")
+    if weights == "fp4" and not model.quantized and len(model.engines):
+        raise EngineError("weights='fp4': the matrices of this model would become four bits in place, and another engine runs them in the compute "
+                          "type: load the weights into another model, or let go of that engine first")
     lines = []
     if kv_cache == "fp4":
         heads = ", ".join(map(str, ops.FP4_HEAD_DIMS))
@@ -109,7 +115,8 @@ class Engine:
     kv_cache: None, keys and values in the compute type; "fp4", in blocks of 32 four-bit numbers that share a power of two
     (``ops.fp4_store``, ``ops.fp4_attention``): 4.25 bits a number, 3.76 times the tokens in the memory of a bfloat16 cache.
     weights: None, the layers' matrices in the compute type; "fp4", in such blocks, the nearest (``ops.fp4_gemm``); the embedding
-    and the head stay as they are.  A loaded model that is handed in is quantized in place.  These kernels are the same whatever ``kernels``.
+    and the head stay as they are.  A loaded model that is handed in is quantized in place, and refused while another engine runs it as it
+    was; a model that is quantized already has to be asked for as such.  These kernels are the same whatever ``kernels``.
     """
 
     def __init__(self, model, dtype="bfloat16", max_tokens: int = 4096, max_seqs: int = 32, page_size: int = 16,
@@ -132,7 +139,7 @@ class Engine:
             check_four_bits(model, kv_cache, weights)
         if weights == "fp4" and not model.quantized:
             model.quantize()
-        self.model, self.kv_cache = model, kv_cache
+        self.model, self.kv_cache, self.weights = model, kv_cache, weights
         self.max_seqs = int(max_seqs)
         if kernels not in ("auto", "plain"):
             raise EngineError(f"kernels={kernels!r}: 'auto' (tuned and fused kernels where they apply) or 'plain'")
@@ -192,6 +199,8 @@ class Engine:
         if graph_decode and not getattr(model, "all_replayable", lambda: False)():
             graph_decode = False
         self.decode_graphs = DecodeGraphs(self) if graph_decode else None
+        if hasattr(model, "engines"):
+            model.engines.add(self)
 
     # ---------------------------------------------------------------- requests
     def has_request(self, request: Hashable) -> bool:

@@ -10,6 +10,7 @@ schedule is simply block i with cache layer i
 """
 from __future__ import annotations
 
+import weakref
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence
 
@@ -90,6 +91,7 @@ class DecoderModel(Part):
         self._taped: Optional[List[bool]] = None       # which blocks let their launches be recorded (parts.tape)
         self.loads = 0                                # times the weights were loaded: recorded tensors are theirs
         self.quantized = False                        # the layers' matrices are held in four bits (``quantize``)
+        self.engines: "weakref.WeakSet" = weakref.WeakSet()   # that run this model: its matrices are theirs as they are
 
     # structure ------------------------------------------------------------------
     def children(self) -> Dict[str, Part]:
@@ -259,7 +261,10 @@ class DecoderModel(Part):
         return [f"{name}: {line}" for line, name in first.items()]
 
     def quantize(self) -> None:
-        """Holds the layers' matrices in four bits, these and any loaded later.  The embedding and the head stay as they are."""
+        """Holds the layers' matrices in four bits, these and any loaded later.  The embedding and the head stay as they are.  Not
+        while an engine runs them in the compute type."""
+        if not self.quantized and len(self.engines):
+            raise RuntimeError("quantize: an engine runs this model with its matrices in the compute type")
         for block in self.blocks:
             block.quantize()
         self.quantized = True
