@@ -137,8 +137,6 @@ class Engine:
         else:
             check_supported(model, self.dtype, self.page_size)
             check_four_bits(model, kv_cache, weights)
-        if weights == "fp4" and not model.quantized:
-            model.quantize()
         self.model, self.kv_cache, self.weights = model, kv_cache, weights
         self.max_seqs = int(max_seqs)
         if kernels not in ("auto", "plain"):
@@ -163,6 +161,8 @@ class Engine:
                 raise EngineError("prefix_caching=True: this model's requests cannot share the pages of a common "
                                   "beginning (build the engine with prefix_caching=False, on the command line "
                                   "--no-prefix-cache):\n  " + "\n  ".join(obstacles))
+        if weights == "fp4" and not model.quantized:
+            model.quantize()    # (in place: only where nothing above has refused the call)
         self.cache = CacheManager(self.page_size, groups, self.max_seqs, bool(prefix_caching))
 
         self.layers: List[LayerCache] = []

@@ -30,3 +30,21 @@ def test_engines_of_both_kinds_of_one_model():
         Engine(model, max_tokens=64, max_seqs=2)
     again = Engine(model, max_tokens=64, max_seqs=2, weights="fp4")
     assert torch.equal(again.step([("a", tokens, [8])]), packed.step([("a", tokens, [8])]))
+
+
+@pytest.mark.parametrize("wrong", [dict(kernels="fast"), dict(prefix_caching=True)])
+def test_a_call_that_is_refused_leaves_the_model_as_it_was(wrong):
+    from glassbox_amd.engine import Engine
+    from glassbox_amd.engine.engine import EngineError
+    from fp4_positions import model_of
+    from glassbox_amd.parts.attention import PagedAttention
+    from glassbox_amd.parts.rotary import Rotary
+    from glassbox_amd.weights.loader import random_tensors
+    model = model_of([Rotary(64, 10000.0)])
+    block = model.blocks[0]
+    block.mixer = PagedAttention(96, 6, 2, 64, Rotary(64, 10000.0), window=20)      # (whose pages cannot be shared)
+    model.load_tree(random_tensors(model, 7, 0.1, "uniform", torch.bfloat16, "cuda:0"))
+    with pytest.raises(EngineError):
+        Engine(model, max_tokens=64, max_seqs=2, kv_cache="fp4", weights="fp4", **wrong)
+    assert not model.quantized and block.mixer.wqkv.dtype == torch.bfloat16
+    Engine(model, max_tokens=64, max_seqs=2)
