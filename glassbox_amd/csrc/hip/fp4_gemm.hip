@@ -67,7 +67,7 @@ __device__ __forceinline__ void put(const GemmArgs& a, int m, int n, int limit, 
 __device__ __forceinline__ void put_or_leave(const GemmArgs& a, int m, int n, int limit, f32x4 v) {
   if (!a.slices) return put(a, m, n, limit, v);
   float* o = a.slices + ((size_t)blockIdx.y * a.M + m) * a.N + n;
-  if (a.N % 4 == 0 && n + 4 <= limit) *reinterpret_cast<f32x4*>(o) = v;
+  if ((a.N | n) % 4 == 0 && n + 4 <= limit) *reinterpret_cast<f32x4*>(o) = v;   // (an up half may begin anywhere)
   else
     for (int i = 0; i < 4 && n + i < limit; ++i) o[i] = v[i];
 }
