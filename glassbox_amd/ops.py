@@ -2610,8 +2610,18 @@ def _stream_of(device: int):
 
 
 def _apart(a0: int, a_rows: int, a_bytes: int, a_step: int, b0: int, b_rows: int, b_bytes: int, b_step: int) -> bool:
-    """Whether two arrays of rows, each from an address on, of so many bytes and as many apart, share no memory."""
-    return a0 + (a_rows - 1) * a_step + a_bytes <= b0 if a0 < b0 else b0 + (b_rows - 1) * b_step + b_bytes <= a0
+    """Whether two arrays of rows, each from an address on, of so many bytes and as many apart, share no memory: one lies behind the other, or
+    their rows lie between each other's (columns of one tensor)."""
+    if (a0 + (a_rows - 1) * a_step + a_bytes <= b0) if a0 < b0 else (b0 + (b_rows - 1) * b_step + b_bytes <= a0):
+        return True
+
+    def meet(d: int, first: int, last: int, step: int) -> bool:   # whether d + k step lies in (-b_bytes, a_bytes) for a k in first..last
+        k = max(first, (-b_bytes - d) // step + 1) if step else first
+        return k <= last and -b_bytes < d + k * step < a_bytes
+
+    if a_step == b_step:   # row j of b begins d + (j - i) step behind row i of a
+        return not meet(b0 - a0, 1 - a_rows, b_rows - 1, a_step)
+    return not any(meet(b0 - a0 - i * a_step, 0, b_rows - 1, b_step) for i in range(a_rows))
 
 
 def fp4_scale_bytes(columns: int) -> int:
