@@ -295,6 +295,7 @@ _SIGS = {
         "gb_fp4_gemm": [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, C.c_longlong, _vp],
         "gb_fp4_gemm_norms": [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, C.c_longlong, _vp, _i, _vp, _i, _vp, _vp, _i, _f, _vp],
         "gb_fp4_gemm_emit_parts": [_i, _i],
+        "gb_fp4_gemm_emit_mode": [_i, _i, _i],
         "gb_fp4_gemm_floats": [_i, _i, _i, _i, _i],
     },
     "sampling": {
