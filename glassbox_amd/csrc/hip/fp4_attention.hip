@@ -581,7 +581,7 @@ static bool takes(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128
 
 // floats of workspace; 0: none is needed
 extern "C" long long gb_fp4_attention_floats(int n_seqs, int nh, int nkv, int hd, int max_q, int max_context, int window, int dtype) {
-  if (n_seqs <= 0 || nkv <= 0 || nh < nkv || max_q <= 0 || max_context <= 0) return 0;
+  if (!takes(hd) || n_seqs <= 0 || nkv <= 0 || nh < nkv || max_q <= 0 || max_context <= 0) return 0;
   const Plan p = plan(n_seqs, nkv, nh / nkv, hd, max_q, max_context, window, dtype);
   return p.splits > 1 ? (long long)n_seqs * nh * max_q * p.splits * (hd + 2) : 0;
 }

@@ -12,3 +12,21 @@ def test_every_entry_point_is_declared():
     used = set(re.findall(r"\.(gb_fp4_\w+)", inspect.getsource(ops)))
     declared = {name for lib in ("fp4_cache", "fp4_attention", "fp4_gemm") for name in ops._SIGS[lib]}
     assert used and used <= declared, used - declared
+
+
+def library(name):
+    """As built, its entry points declared (``ops`` asks for a GPU before it loads one)"""
+    lib = build.load(name)
+    for fn, args in ops._SIGS[name].items():
+        getattr(lib, fn).argtypes = args
+        getattr(lib, fn).restype = ctypes.c_longlong if fn.endswith("_floats") else ctypes.c_int
+    lib.gb_last_error.restype = ctypes.c_char_p
+    return lib
+
+
+@pytest.mark.parametrize("hd", [-64, 0, 16, 48, 160, 288, 320, 512, 1 << 20])
+def test_heads_that_attention_does_not_take_need_no_workspace(hd):
+    """(The model of the launches' times has numbers for the heads that it takes alone.)"""
+    floats = library("fp4_attention").gb_fp4_attention_floats
+    assert floats(1, 32, 8, 128, 300, 16000, 0, ops.BF16) > 0
+    assert floats(1, 32, 8, hd, 300, 16000, 0, ops.BF16) == 0 and floats(1, 32, 8, hd, 1, 16000, 0, ops.F32) == 0
