@@ -603,7 +603,8 @@ extern "C" int gb_fp4_attention(const void* q, int q_stride, void* out, int out_
   const int rep = nh / nkv;
   const Plan p = plan(n_seqs, nkv, rep, hd, max_q, std::max(1, max_context), window, dtype);
   const long long columns = (long long)n_seqs * nh * max_q, groups = (long long)n_seqs * nkv * p.col_tiles * p.splits;
-  GB_REQUIRE(columns < (1ll << 31) && groups < (1ll << 31), "fp4_attention: too many rows for one launch");
+  // (a last workgroup's columns, up to 192 and most of them none of the request's, have numbers of 32 bits too)
+  GB_REQUIRE(columns <= INT32_MAX - 1024 && groups < (1ll << 31), "fp4_attention: too many rows for one launch");
   const long long need = p.splits > 1 ? columns * p.splits * (hd + 2) : 0;
   GB_REQUIRE(need == 0 || (workspace && workspace_floats >= need), "fp4_attention: a workspace of %lld floats is needed, %lld are given", need,
              workspace ? workspace_floats : 0ll);
