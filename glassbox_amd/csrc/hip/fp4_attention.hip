@@ -27,6 +27,7 @@
 namespace gb {
 
 constexpr int kTile = 64;        // keys a wave takes at a time
+constexpr float kLargest = 3.402823466e38f;
 constexpr int kMostSplits = 64;  // runs of a context: a lane each in the kernel that joins them
 
 struct AttendArgs {
@@ -91,6 +92,9 @@ __device__ __forceinline__ Places look_up(const AttendArgs& a, const int32_t* ta
 }
 // the first key that a window leaves a position; no sum passes 32 bits, whatever the position
 __device__ __forceinline__ int window_from(const AttendArgs& a, int pos) { return a.window > 0 ? max(pos, a.window - 1) - (a.window - 1) : 0; }
+// What a column's sum of p v is multiplied by: zeros for one that sees no key (its maximum is still minus infinity), NaN for one all of whose
+// keys have scores of minus infinity.
+__device__ __forceinline__ float over_sum(float sum, float m) { return sum > 0.f || sum != sum ? 1.f / sum : m == -__builtin_inff() ? 0.f : __builtin_nanf(""); }
 // a page of the pool; page 0 in the place of any other number, which is not read
 __device__ __forceinline__ bool known_page(const AttendArgs& a, int page) { return (unsigned)page < (unsigned)a.pages; }
 __device__ __forceinline__ size_t page_at(const AttendArgs& a, int page, int kvh, size_t head_bytes) {
@@ -128,19 +132,20 @@ __device__ __forceinline__ uint32_t mask_scores(f32x4 (&sc)[4], int key, bool kn
   return seen;
 }
 
-// One step of the running softmax of a column (this lane's 16 keys of 64): probabilities as the product's operand, sums rescaled where
-// the maximum grows.  Their sum is a product with ones, of what the values are multiplied by and over all 64 (added up by the lanes: 64 requests of
+// One step of the running softmax of a column (this lane's 16 keys of 64, of which it sees `seen`): probabilities as the product's operand, sums rescaled
+// where the maximum grows.  The maximum is that of the scores as they are, not scaled.  Scaled it is rounded, which numerator and denominator share: by
+// up to 2^32 up to 2^29, where scores that differ at all are 2^32 apart already and any larger multiplier will do.  Their sum is a product with ones, of what the values are multiplied by and over all 64 (added up by the lanes: 64 requests of
 // 4,096 keys 136 us for 126, 2,048 rows of 32 heads of 128 72.5 for 73).  PT terms a probability.
 template <int PT, int NB>
-__device__ __forceinline__ void soften(const f32x4 (&sc)[4], float scale, float& m, f32x4& l, f32x4 (&o)[2 * NB], bf16x8 (&pf)[PT][2]) {
-  float top = -__builtin_inff();
+__device__ __forceinline__ void soften(const f32x4 (&sc)[4], uint32_t seen, float scale, float& m, f32x4& l, f32x4 (&o)[2 * NB], bf16x8 (&pf)[PT][2]) {
+  float top = seen ? -kLargest : -__builtin_inff();
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int x = 0; x < 4; ++x) top = fmaxf(top, sc[j][x]);
-  const float now = fmaxf(m, quads_max(top) * scale);   // (the scale is positive)
+  const float now = fmaxf(m, quads_max(top));   // (the scale is positive)
   if (__any(now > m)) {
-    const float shrink = now > m ? __builtin_amdgcn_exp2f(m - now) : 1.f;
+    const float shrink = now > m ? __builtin_amdgcn_exp2f((m - now) * scale) : 1.f;
     m = now;
     l[0] *= shrink;
 #pragma unroll
@@ -148,12 +153,14 @@ __device__ __forceinline__ void soften(const f32x4 (&sc)[4], float scale, float&
 #pragma unroll
       for (int x = 0; x < 4; ++x) o[b][x] *= shrink;
   }
-  const float sub = m == -__builtin_inff() ? 0.f : m;
+  // what the scores are multiplied by: the scale, or where that brings the maximum beyond 2^29 the power of two that brings it there
+  const float by = fminf(scale, __uint_as_float((283u << 23) - max(__float_as_uint(m) & 0x7f800000u, 29u << 23)));
+  const float sub = m == -__builtin_inff() ? 0.f : m * by;
   float p[16];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) p[4 * j + x] = __builtin_amdgcn_exp2f(fmaf(sc[j][x], scale, -sub));
+    for (int x = 0; x < 4; ++x) p[4 * j + x] = __builtin_amdgcn_exp2f(fmaf(sc[j][x], by, -sub));
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     float x[8];
@@ -305,7 +312,7 @@ template <typename T, int NB, int R> struct Columns {
     }
     bf16x8 pf[R][PT][2];
 #pragma unroll
-    for (int t = 0; t < R; ++t) soften<PT, NB>(sc[t], a.scale, m[t], l[t], o[t], pf[t]);
+    for (int t = 0; t < R; ++t) soften<PT, NB>(sc[t], seen[t], a.scale, m[t], l[t], o[t], pf[t]);
     if (__builtin_expect(bad, 0)) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
@@ -390,7 +397,7 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least
   for (int w = 1; w < W; ++w) top = fmaxf(top, sm[w][column]);
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    weight[w] = sm[w][column] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sm[w][column] - top);
+    weight[w] = sm[w][column] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((sm[w][column] - top) * a.scale);
     sum += weight[w] * sl[w][column];
   }
   float x[kEach];
@@ -406,7 +413,7 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least
 #pragma unroll
     for (int e = 0; e < kEach; ++e) a.acc[to * D + part * kEach + e] = x[e];
   } else {
-    const float over = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const float over = over_sum(sum, top);
     T* row = (T*)a.out + (size_t)(q_start + c / a.rep) * a.out_stride + (size_t)(kvh * a.rep + c % a.rep) * D;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) row[part * kEach + e] = (T)(x[e] * over);
@@ -462,7 +469,7 @@ __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(least
 #pragma unroll
       for (int b = 0; b < 2 * NB; ++b) *reinterpret_cast<f32x4*>(a.acc + to * D + 16 * b + 4 * g) = columns.o[t][b];
     } else {
-      const float over = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+      const float over = over_sum(sum, columns.m[t]);
       T* row = (T*)a.out + (size_t)(q_start + c / a.rep) * a.out_stride + (size_t)(kvh * a.rep + c % a.rep) * D;
 #pragma unroll
       for (int b = 0; b < 2 * NB; ++b) {
@@ -485,8 +492,8 @@ __global__ __launch_bounds__(256) void fp4_join_kernel(AttendArgs a, int columns
   if (q_start < 0 || token >= min(a.q_len[s], a.n - q_start)) return;
   const float2 ml = lane < a.splits ? a.ml[(size_t)at * a.splits + lane] : make_float2(-__builtin_inff(), 0.f);
   const float top = wave_max(ml.x);
-  const float weight = ml.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
-  const float sum = wave_sum(weight * ml.y), over = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  const float weight = ml.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((ml.x - top) * a.scale);
+  const float sum = wave_sum(weight * ml.y), over = over_sum(sum, top);
   constexpr int kEach = (D + kWave - 1) / kWave;
   float x[kEach] = {};
   // (runs in which a column sees nothing have left zeros; what is read again behind the last has no weight)
