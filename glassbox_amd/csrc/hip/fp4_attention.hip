@@ -117,17 +117,17 @@ template <typename T, int NB> __device__ __forceinline__ void load_query(const T
     }
 }
 
-// Scores of 16 keys from `key` on that the column does not see become minus infinity; the bits of those it sees.
+// Scores of 16 keys from `key` on that the column does not see become minus infinity; the bits of those it sees.  (The bits first, then a score at a time
+// by its bit: sixteen comparisons kept as they are spill 63 to 85 scalar registers.)
 __device__ __forceinline__ uint32_t mask_scores(f32x4 (&sc)[4], int key, bool known, int from, int pos, int end) {
-  uint32_t seen = 0;
+  const int first = min(max(from - key, 0), 16), last = known ? min(max(min(pos, end - 1) - key + 1, first), 16) : first;
+  const uint32_t seen = (1u << last) - (1u << first);
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const int k = key + 4 * j + x;
-      const bool in = known && k >= from && k <= pos && k < end;
-      seen |= in ? 1u << (4 * j + x) : 0u;
-      sc[j][x] = in ? sc[j][x] : -__builtin_inff();
+      const uint32_t in = (uint32_t)__builtin_amdgcn_sbfe((int)seen, 4 * j + x, 1);   // all bits or none
+      sc[j][x] = __uint_as_float((__float_as_uint(sc[j][x]) & in) | (0xff800000u & ~in));
     }
   return seen;
 }
