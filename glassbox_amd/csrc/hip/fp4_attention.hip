@@ -15,7 +15,7 @@
 // Codes become bf16 in registers, two an instruction with their scale, exactly; nothing passes through LDS but the joining of waves.
 // A row of 32 bits counts as three bf16 terms (fp4.h), and so do its probabilities.  Those of a bf16 row count as two, off by 2^-16: its
 // result is rounded once, at the end.  (As one term they were off by 2^-8: the distance from the 64-bit definition was 0.0021 of the results where their
-// own rounding is 0.0016, and far more of sums that cancel; it took 4 to 6 % less time for single tokens, 12 to 17 % less for portions.)
+// own rounding is 0.0016, and far more of sums that cancel; it takes 2 to 7 % less time for single tokens, 11 to 15 % less for portions.)
 //
 // Few columns (decoding): the waves of a workgroup share out the tiles and are joined through LDS; a long context is cut into runs
 // for several workgroups, joined by a second kernel.  More columns: each wave has columns of its own and all of a run's keys.
@@ -135,7 +135,7 @@ __device__ __forceinline__ uint32_t mask_scores(f32x4 (&sc)[4], int key, bool kn
 // One step of the running softmax of a column (this lane's 16 keys of 64, of which it sees `seen`): probabilities as the product's operand, sums rescaled
 // where the maximum grows.  The maximum is that of the scores as they are, not scaled.  Scaled it is rounded, which numerator and denominator share: by
 // up to 2^32 up to 2^29, where scores that differ at all are 2^32 apart already and any larger multiplier will do.  Their sum is a product with ones, of what the values are multiplied by and over all 64 (added up by the lanes: 64 requests of
-// 4,096 keys 136 us for 126, 2,048 rows of 32 heads of 128 72.5 for 73).  PT terms a probability.
+// 4,096 keys 120 us for 118, 2,048 rows of 32 heads of 128 72.5 for 71.8).  PT terms a probability.
 template <int PT, int NB>
 __device__ __forceinline__ void soften(const f32x4 (&sc)[4], uint32_t seen, float scale, float& m, f32x4& l, f32x4 (&o)[2 * NB], bf16x8 (&pf)[PT][2]) {
   float top = seen ? -kLargest : -__builtin_inff();
@@ -345,11 +345,11 @@ template <typename T, int NB, int R> struct Columns {
 };
 
 // Waves a SIMD holds at least: what just fits the registers.  (Without the bound a few more registers cost a wave: 64 requests of 4,096 keys, 32 heads of
-// 64, 158 us, with it 127; 2,048 rows of 32 heads of 128 108 and 73.)
+// 64, 120 us, with it 118; 2,048 rows of 32 heads of 128 107 and 72.)
 template <typename T, int NB, int R> constexpr int least_waves = NB > 4 ? 1 : std::is_same_v<T, float> || R > 1 ? 2 : NB > 2 ? 3 : 4;
 
 // Few columns: the waves of a workgroup share out the tiles of keys.  T the rows' type, NB blocks a head, W waves.  Bound by memory: 64 requests of
-// 4,096 keys, 32 heads of 64, 127 us for 571 MB (4.5 TB/s); 64 of 4,000, 8 kv heads of 128, 62 us (4.5 TB/s).
+// 4,096 keys, 32 heads of 64, 118 to 123 us for 571 MB (4.7 TB/s); 64 of 4,000, 8 kv heads of 128, 60 us (4.7 TB/s).
 template <typename T, int NB, int W>
 __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least_waves<T, NB, 1>))) void fp4_attend_keys_kernel(AttendArgs a) {
   constexpr int D = NB * kFp4Block;
@@ -421,8 +421,8 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least
 }
 
 // More columns: each of four waves has R tiles of its own and takes all keys.  Bound by the conversions, the softmax and the products, which add up: 2,048
-// rows of 32 heads of 128 in 73 us (the same rows over a bf16 cache in the prefill kernel: 56).  A request's long tiles of columns come first and its
-// short ones behind them in turn, so that compute units of two workgroups have about the same to do: in their order 93.  Making a tile bf16 once for
+// rows of 32 heads of 128 in 72 us (the same rows over a bf16 cache in the prefill kernel: 56).  A request's long tiles of columns come first and its
+// short ones behind them in turn, so that compute units of two workgroups have about the same to do: in their order 92.  Making a tile bf16 once for
 // the four waves, through LDS, took half as long again (95 for 64, with probabilities of one term): the barriers cost more than the conversions that they save.
 template <typename T, int NB, int R>
 __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(least_waves<T, NB, R>))) void fp4_attend_cols_kernel(AttendArgs a) {
@@ -528,9 +528,9 @@ static Plan plan(int n_seqs, int nkv, int rep, int hd, int max_q, int max_contex
     return Plan{cols, r, (int)((columns + width - 1) / width), (int)std::max<long long>(1, (span + chunk - 1) / chunk), (int)chunk};
   };
   // Few columns, runs of a context: as many workgroups as compute units have one, none of fewer than 512 keys; 129 to 217 workgroups of long contexts
-  // in three.  Over 110 sizes 1.6 % slower than the best number of runs.  us: one request of 4,000 keys and 32 kv heads in 8 runs 9.8, in 4 11.3;
-  // 256 workgroups in one run 20.0, in two 23.3; 160 (5 of 9,000) in three 30.5, in two 39.3.  More than 256 stay whole: 40 requests of 1,000 to 8,000 keys
-  // and 8 kv heads 65.8, in three 66.4, though 10 of 9,000 and 32 kv heads take 65.7 and 52.5.
+  // in three.  Over 110 sizes 1.6 % slower than the best number of runs.  us: one request of 4,000 keys and 32 kv heads in 8 runs 9.2, in 4 10.7;
+  // 256 workgroups in one run 19.4, in two 22.1; 160 (5 of 9,000) in three 29.2, in two 37.6.  More than 256 stay whole: 40 requests of 1,000 to 8,000 keys
+  // and 8 kv heads 62.2, in three 61.8, though 10 of 9,000 and 32 kv heads take 60.6 and 49.1.
   if (columns <= 32) {
     const long long groups = (long long)n_seqs * nkv * ((columns + 15) / 16);
     long long runs = std::max<long long>(1, std::min<long long>(256 / groups, kMostSplits));
@@ -538,19 +538,19 @@ static Plan plan(int n_seqs, int nkv, int rep, int hd, int max_q, int max_contex
     if (max_context <= 1024) runs = 1;
     return laid_out(false, 1, runs, 512, 8 * kTile);
   }
-  // More: one tile of columns a wave, two (where they fit the registers) or three (heads of 64: of 32 they gain nothing), and as many runs, as take least by a model with numbers fitted to some 2,000
-  // launches (of probabilities of one term; its choice is 3 % slower than the best over 64 sizes, at most 20): a wave's turns, each `alone` us; the tiles that a
-  // SIMD has to do on average, `busy` us each, more where the workgroups do not divide evenly by the compute units; the joining of runs, its launch and its
-  // bytes.  us: 131 rows behind 3,900, 32 heads of 64 and as many kv heads, three tiles in 8 runs 27.1, two in 11 27.9, one in 11 33.4; 8 kv heads of 128 two
-  // in 6 36.3, in 8 43.7; 1,024 rows of 32 heads of 64 two in one run 27.4, in two 42.3, though one in one takes 22.9; 8 x 50 rows behind 550 one in one
-  // 22.6, two in two 29.1; 131 rows behind 15,869, 32 heads of 64, three in 23 65.4, two in 16 76.7; 300 behind 15,700 three in 12 115, two in 16 124.
-  static constexpr float kAlone[3][9] = {{0.f, 0.38f, 0.48f, 1.2f, 0.75f, 0.f, 0.f, 0.f, 1.f}, {0.f, 0.55f, 0.59f, 1.35f, 1.01f}, {0.f, 0.f, 0.89f}};   // by tiles and blocks a head
-  static constexpr float kBusy[3][9] = {{0.f, 0.52f, 0.65f, 1.1f, 0.84f, 0.f, 0.f, 0.f, 2.2f}, {0.f, 0.59f, 0.8f, 1.2f, 0.91f}, {0.f, 0.f, 0.9f}};
+  // More: one tile of columns a wave, two (where they fit the registers) or three (heads of 64: of 32 they gain nothing), and as many runs, as take least by a model with numbers fitted to some 3,000
+  // launches (154 sizes: its choice is 1.5 % slower than the best, at most 19): a wave's turns, each `alone` us; the tiles that a SIMD has to do on
+  // average, `busy` us each, more where the workgroups do not divide evenly by the compute units; the joining of runs, its launch and its
+  // bytes.  us: 131 rows behind 3,900, 32 heads of 64 and as many kv heads, three tiles in 8 runs 27.0, in 16 27.4, two in 11 27.7, one in 11 29.6; 8 kv
+  // heads of 128 two in 6 35.5, in 8 44.3, one in 11 38.2; 1,024 rows of 32 heads of 64 one in one run 19.7, two 27.1; 2,048 rows of 32 heads of 64 two in one
+  // 53, one 59; 8 x 50 rows behind 550 one in one 20.3, two in two 27.8; 131 rows behind 15,869, 32 heads of 64, three in 16 64.8, two 75.8, one 77.3.
+  static constexpr float kAlone[3][9] = {{0.f, 0.38f, 0.48f, 1.2f, 0.75f, 0.f, 0.f, 0.f, 1.f}, {0.f, 0.61f, 0.65f, 1.49f, 1.11f}, {0.f, 0.f, 1.2f}};   // by tiles and blocks a head
+  static constexpr float kBusy[3][9] = {{0.f, 0.57f, 0.72f, 1.21f, 0.92f, 0.f, 0.f, 0.f, 2.42f}, {0.f, 0.89f, 1.2f, 1.8f, 1.36f}, {0.f, 0.f, 1.08f}};
   const bool wide = dtype == kF32;
   Plan best{};
   float least = 0.f;
   for (int r = 1; r <= (wide || hd > 128 ? 1 : hd == 64 ? 3 : 2); ++r) {
-    const float alone = kAlone[r - 1][hd / 32] * (wide ? 1.25f : 1.f), busy = kBusy[r - 1][hd / 32] * (wide ? 1.65f : 1.f);
+    const float alone = kAlone[r - 1][hd / 32] * (wide ? 1.4f : 1.f), busy = kBusy[r - 1][hd / 32] * (wide ? 1.4f : 1.f);
     const float waves = (float)n_seqs * nkv * (float)((columns + 16 * r - 1) / (16 * r));
     for (int runs : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64}) {
       const Plan p = laid_out(true, r, runs, kTile, kTile);
