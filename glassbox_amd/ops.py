@@ -2732,7 +2732,7 @@ def fp4_attention(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_l
     last so many) through ``tables`` int32 [requests, pages], and ``out`` receives its rows.  Rows of no request are left as they are.
     ``max_q_len`` and ``max_context`` are at least the most rows and keys a request has; they size the launch.  A row that sees no key (its
     position is negative, its pages' numbers are none of the pool's) gives zeros; what lies in a masked place, not finite or not, does not
-    matter.  bfloat16 or float32 rows; heads of 32, 64, 96, 128 or 256 channels; a positive scale.
+    matter.  Scores may be of any size; a row that sees keys, all with scores of minus infinity, gives NaN.  bfloat16 or float32 rows; heads of 32, 64, 96, 128 or 256 channels; a positive scale.
     ``workspace`` (float32, ``fp4_attention_floats`` elements): needed where that is not 0."""
     pages, nkv, page_size, hd, k_at, v_at = _fp4_pages(k_pages, v_pages, "fp4_attention")
     q_stride, out_stride, shape = _rows(q, "q"), _rows(out, "out"), q.shape
