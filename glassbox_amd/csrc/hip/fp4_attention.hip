@@ -133,9 +133,10 @@ __device__ __forceinline__ uint32_t mask_scores(f32x4 (&sc)[4], int key, bool kn
 }
 
 // One step of the running softmax of a column (this lane's 16 keys of 64, of which it sees `seen`): probabilities as the product's operand, sums rescaled
-// where the maximum grows.  The maximum is that of the scores as they are, not scaled.  Scaled it is rounded, which numerator and denominator share: by
-// up to 2^32 up to 2^29, where scores that differ at all are 2^32 apart already and any larger multiplier will do.  Their sum is a product with ones, of what the values are multiplied by and over all 64 (added up by the lanes: 64 requests of
-// 4,096 keys 120 us for 118, 2,048 rows of 32 heads of 128 72.5 for 71.8).  PT terms a probability.
+// where the maximum grows.  The maximum is that of the scores as they are, and what is scaled is their difference: a scaled maximum is rounded, by 2^-4 at
+// 2^20 and 2^32 at 2^56, which the probabilities of a tile share, but not those of the next one.  (One operation a score more than scores scaled by the
+// multiplication that subtracts: 2,048 rows of 32 heads of 128 73.5 us for 72.2.)  Their sum is a product with ones, of what the values are multiplied by
+// and over all 64 (added up by the lanes: 64 requests of 4,096 keys 120 us for 118, the prompt 72.5 for 71.8).  PT terms a probability.
 template <int PT, int NB>
 __device__ __forceinline__ void soften(const f32x4 (&sc)[4], uint32_t seen, float scale, float& m, f32x4& l, f32x4 (&o)[2 * NB], bf16x8 (&pf)[PT][2]) {
   float top = seen ? -kLargest : -__builtin_inff();
@@ -153,14 +154,12 @@ __device__ __forceinline__ void soften(const f32x4 (&sc)[4], uint32_t seen, floa
 #pragma unroll
       for (int x = 0; x < 4; ++x) o[b][x] *= shrink;
   }
-  // what the scores are multiplied by: the scale, or where that brings the maximum beyond 2^29 the power of two that brings it there
-  const float by = fminf(scale, __uint_as_float((283u << 23) - max(__float_as_uint(m) & 0x7f800000u, 29u << 23)));
-  const float sub = m == -__builtin_inff() ? 0.f : m * by;
+  const float least = m == -__builtin_inff() ? 0.f : m;
   float p[16];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) p[4 * j + x] = __builtin_amdgcn_exp2f(fmaf(sc[j][x], by, -sub));
+    for (int x = 0; x < 4; ++x) p[4 * j + x] = __builtin_amdgcn_exp2f((sc[j][x] - least) * scale);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     float x[8];

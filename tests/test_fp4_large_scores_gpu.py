@@ -63,3 +63,34 @@ def test_rows_that_see_no_key_are_zeros_whatever_their_queries():
         assert (out == 0).all()
         ops.fp4_attention(q, out.fill_(5.0), ints([0]), ints([rows]), ints([0]), ints([[-1, 7]]), kp, kp.clone(), 4, 0.125, rows, 64)
         assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,G,D,rows", [(4, 4, 64, 1), (8, 1, 128, 1), (8, 2, 32, 40), (32, 32, 64, 130), (32, 8, 128, 200), (4, 2, 256, 40)])
+@pytest.mark.parametrize("step,scale", [(2.0 ** -10, 1e3), (2.0 ** -20, 1e6), (2.0 ** -23, 1e7)])
+@pytest.mark.parametrize("longest", [256, 20000])
+def test_differences_that_are_small_beside_the_scores(H, G, D, rows, dtype, step, scale, longest):
+    """Scores of 1 and, every other run of 64 keys, 1 + step, exactly; their difference, scaled, is about 1, the scores themselves 10^3 to 10^7: what
+    a tile's maximum loses by a rounding, the next tile's does not.  The bound is that of the test above; the scaled difference is off by 2^-23
+    of itself, at most 2."""
+    from glassbox_amd import ops
+    keys, page = 256, 16
+    k, v = torch.zeros(keys, G, D), torch.zeros(keys, G, D)
+    upper = torch.arange(keys) // 64 % 2 == 1
+    k[..., 3] = 1
+    k[upper, :, 4] = 1
+    v[...], v[upper] = 1, 3
+    kp, vp = torch.zeros(2, *ops.fp4_pages_shape(keys // page, G, page, D), dtype=torch.uint8, device=DEV)
+    ops.fp4_store(torch.cat([k.flatten(1), v.flatten(1)], 1).to(DEV), None, None, torch.arange(keys, dtype=torch.int32, device=DEV), kp, vp, 0, G, D)
+    q = torch.zeros(rows, H, D)
+    q[..., 3], q[..., 4] = 1, step
+    table = torch.arange(keys // page, dtype=torch.int32, device=DEV)[None]
+    ints = lambda x: torch.tensor([x], dtype=torch.int32, device=DEV)
+    floats = ops.fp4_attention_floats(1, H, G, D, rows, longest, 0, dtype)
+    out = torch.empty(rows, H * D, dtype=dtype, device=DEV)
+    ops.fp4_attention(q.to(dtype).flatten(1).to(DEV), out, ints(0), ints(rows), ints(keys - 1), table, kp, vp, H, scale, rows, longest,
+                      workspace=torch.empty(floats, device=DEV) if floats else None)
+    weight = math.exp(step * scale)
+    want = (1 + 3 * weight) / (1 + weight)
+    bound = torch.finfo(dtype).eps / 2 * want + 3 * (2 * 2 ** -16 + 2 * keys * 2 ** -23 + 2 ** -21)
+    assert (out.double() - want).abs().max().item() <= bound
