@@ -15,7 +15,7 @@
 // Codes become bf16 in registers, two an instruction with their scale, exactly; nothing passes through LDS but the joining of waves.
 // A row of 32 bits counts as three bf16 terms (fp4.h), and so do its probabilities.  Those of a bf16 row count as two, off by 2^-16: its
 // result is rounded once, at the end.  (As one term they were off by 2^-8: the distance from the 64-bit definition was 0.0021 of the results where their
-// own rounding is 0.0016, and far more of sums that cancel; it takes 2 to 7 % less time for single tokens, 11 to 15 % less for portions.)
+// own rounding is 0.0016, and far more of sums that cancel; it takes 3 to 9 % less time for single tokens, 9 to 16 % less for portions.)
 //
 // Few columns (decoding): the waves of a workgroup share out the tiles and are joined through LDS; a long context is cut into runs
 // for several workgroups, joined by a second kernel.  More columns: each wave has columns of its own and all of a run's keys.
@@ -136,7 +136,7 @@ __device__ __forceinline__ uint32_t mask_scores(f32x4 (&sc)[4], int key, bool kn
 // where the maximum grows.  The maximum is that of the scores as they are, and what is scaled is their difference: a scaled maximum is rounded, by 2^-4 at
 // 2^20 and 2^32 at 2^56, which the probabilities of a tile share, but not those of the next one.  (One operation a score more than scores scaled by the
 // multiplication that subtracts: 2,048 rows of 32 heads of 128 73.5 us for 72.2.)  Their sum is a product with ones, of what the values are multiplied by
-// and over all 64 (added up by the lanes: 64 requests of 4,096 keys 120 us for 118, the prompt 72.5 for 71.8).  PT terms a probability.
+// and over all 64 (added up by the lanes: 64 requests of 4,096 keys 123 us for 122, the prompt 74.0 for 73.7).  PT terms a probability.
 template <int PT, int NB>
 __device__ __forceinline__ void soften(const f32x4 (&sc)[4], uint32_t seen, float scale, float& m, f32x4& l, f32x4 (&o)[2 * NB], bf16x8 (&pf)[PT][2]) {
   float top = seen ? -kLargest : -__builtin_inff();
@@ -344,11 +344,11 @@ template <typename T, int NB, int R> struct Columns {
 };
 
 // Waves a SIMD holds at least: what just fits the registers.  (Without the bound a few more registers cost a wave: 64 requests of 4,096 keys, 32 heads of
-// 64, 120 us, with it 118; 2,048 rows of 32 heads of 128 107 and 72.)
+// 64, 124 us, with it 122; 2,048 rows of 32 heads of 128 110 and 74.)
 template <typename T, int NB, int R> constexpr int least_waves = NB > 4 ? 1 : std::is_same_v<T, float> || R > 1 ? 2 : NB > 2 ? 3 : 4;
 
 // Few columns: the waves of a workgroup share out the tiles of keys.  T the rows' type, NB blocks a head, W waves.  Bound by memory: 64 requests of
-// 4,096 keys, 32 heads of 64, 118 to 123 us for 571 MB (4.7 TB/s); 64 of 4,000, 8 kv heads of 128, 60 us (4.7 TB/s).
+// 4,096 keys, 32 heads of 64, 119 to 125 us for 571 MB (4.7 TB/s); 64 of 4,000, 8 kv heads of 128, 61 us (4.6 TB/s).
 template <typename T, int NB, int W>
 __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least_waves<T, NB, 1>))) void fp4_attend_keys_kernel(AttendArgs a) {
   constexpr int D = NB * kFp4Block;
@@ -420,8 +420,8 @@ __global__ __launch_bounds__(W * kWave) __attribute__((amdgpu_waves_per_eu(least
 }
 
 // More columns: each of four waves has R tiles of its own and takes all keys.  Bound by the conversions, the softmax and the products, which add up: 2,048
-// rows of 32 heads of 128 in 72 us (the same rows over a bf16 cache in the prefill kernel: 56).  A request's long tiles of columns come first and its
-// short ones behind them in turn, so that compute units of two workgroups have about the same to do: in their order 92.  Making a tile bf16 once for
+// rows of 32 heads of 128 in 73 us (the same rows over a bf16 cache in the prefill kernel: 56).  A request's long tiles of columns come first and its
+// short ones behind them in turn, so that compute units of two workgroups have about the same to do: in their order 94.  Making a tile bf16 once for
 // the four waves, through LDS, took half as long again (95 for 64, with probabilities of one term): the barriers cost more than the conversions that they save.
 template <typename T, int NB, int R>
 __global__ __launch_bounds__(4 * kWave) __attribute__((amdgpu_waves_per_eu(least_waves<T, NB, R>))) void fp4_attend_cols_kernel(AttendArgs a) {
